@@ -41,12 +41,23 @@ def build(verbose: bool = False):
                 os.path.basename(h)[:-4] + ".cuda.o")
             if os.path.exists(obj):
                 os.remove(obj)
+    # ninja does not track the .hip sources' headers either: an object
+    # older than any of them is compiled again
+    newest = max(os.path.getmtime(h)
+                 for h in glob.glob(os.path.join(CSRC, "*.h")))
+    for obj in glob.glob(os.path.join(PKG_DIR, "*.o")):
+        if os.path.getmtime(obj) < newest:
+            os.remove(obj)
     mod = load(
         name="_dlb_kernels",
         sources=sources,
         build_directory=PKG_DIR,
         extra_cflags=["-O3"],
-        extra_cuda_cflags=["-O3", "--offload-arch=gfx950"],
+        # no packed fp32 arithmetic (v_pk_add/mul/fma_f32): some of its
+        # forms have given wrong results on this hardware
+        extra_cuda_cflags=["-O3", "--offload-arch=gfx950",
+                           "-Xclang", "-target-feature",
+                           "-Xclang", "-packed-fp32-ops"],
         verbose=verbose,
     )
     # guard against a stale incremental link silently dropping a newly
