@@ -63,7 +63,8 @@ def build(verbose: bool = False):
     # guard against a stale incremental link silently dropping a newly
     # added source (observed once with the ninja/hipify cache)
     for attr in ("conv_fwd", "gn_bwd", "lmloss_fwd", "se_fwd", "dropout",
-                 "embed_fwd", "gn_dgb_reduce_multi", "attn_fwd"):
+                 "embed_fwd", "gn_dgb_reduce_multi", "attn_fwd",
+                 "packed_attn_bwd", "relbias_bwd"):
         if not hasattr(mod, attr):
             raise RuntimeError(
                 f"_dlb_kernels is missing `{attr}` after build — stale "

@@ -967,7 +967,10 @@ static std::vector<torch::Tensor> se_bwd(torch::Tensor x, torch::Tensor g,
   return {dx, dg};
 }
 
+void bind_longctx(py::module_& m);  // longctx_bindings.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  bind_longctx(m);
   m.def("conv_fwd", &conv_fwd, "Implicit-GEMM NHWC bf16 conv forward");
   m.def("conv_bwd_data", &conv_bwd_data, "NHWC bf16 conv input-grad",
         py::arg("dy"), py::arg("w"), py::arg("IH"), py::arg("IW"),

@@ -14,16 +14,20 @@ coverage from it.
 
 from __future__ import annotations
 
+import math
+
 import torch
 import torch.nn.functional as F
 
 from . import available, ext
+from .packing import PackedSequences, checked_starts  # noqa: F401
 
 # ops with a hand-written gfx950 kernel wired in (grown as kernels land)
 NATIVE_OPS: set[str] = {"group_norm_act", "conv2d", "layer_norm",
                         "causal_attention", "avg_pool2d", "log_softmax",
                         "max_pool2d", "lm_loss", "dropout", "embedding",
-                        "se_mul"}
+                        "se_mul", "packed_causal_attention",
+                        "relative_position_bias"}
 
 
 def _use_native(name: str, x: torch.Tensor) -> bool:
@@ -190,6 +194,158 @@ def causal_attention(q, k, v, nhead, dropout_p=0.0, training=False):
     out = F.scaled_dot_product_attention(
         split(q), split(k), split(v), dropout_p=pd, is_causal=True)
     return out.transpose(0, 1).reshape(S, B, E)
+
+
+def relative_position_bias(table, q_len, k_len, max_distance=128,
+                           bidirectional=False):
+    """Learned bias by bucketed distance: [nhead, q_len, k_len].
+
+    out[h, i, j] = table[bucket(i + k_len - q_len - j), h] with ``table``
+    [num_buckets, nhead] (bf16, fp16 or fp32; the result has its type, the
+    autocast type under autocast).  The queries are the last ``q_len`` of
+    the ``k_len`` positions, so one generated token is ``q_len=1``.
+
+    Half of the buckets hold one distance each, the others divide the
+    logarithm up to ``max_distance`` evenly, and the last takes all that is
+    farther.  ``bidirectional`` gives keys ahead of the query the second
+    half of the buckets; without it they count as distance 0.  The gradient
+    of ``table`` is summed in fp32 in a fixed order.
+    """
+    if table.dim() != 2:
+        raise ValueError("the bias table is [num_buckets, nhead], got "
+                         f"{tuple(table.shape)}")
+    if table.dtype not in (torch.bfloat16, torch.float16, torch.float32,
+                           torch.float64):
+        raise TypeError(f"the bias table has to be floating, "
+                        f"got {table.dtype}")
+    if q_len < 0 or k_len < 0:
+        raise ValueError("lengths must not be negative")
+    starts = checked_starts(table.shape[0], max_distance, bidirectional)
+    if _use_native("relative_position_bias", table):
+        if table.dtype == torch.float64:
+            raise TypeError("the position bias runs in bf16, fp16 or fp32 "
+                            "on the GPU")
+        from . import native
+        return native.relative_position_bias(table, q_len, k_len, starts)
+    n = (torch.arange(q_len, device=table.device)[:, None] + (k_len - q_len)
+         - torch.arange(k_len, device=table.device))
+    edges = torch.tensor(starts, device=table.device)
+    bucket = torch.bucketize(n.abs() if bidirectional else n.clamp(min=0),
+                             edges, right=True) - 1
+    if bidirectional:
+        bucket = bucket + (n < 0) * len(starts)
+    return table.t()[:, bucket]
+
+
+def packed_causal_attention(q, k, v, packing, scale=None, bias_table=None,
+                            max_distance=128):
+    """Causal self-attention over sequences packed behind each other.
+
+    ``q`` [T, nhead, d], ``k`` and ``v`` [T, kv_heads, d]; query heads
+    ``h`` with the same ``h // (nhead // kv_heads)`` share a key/value
+    head.  ``packing`` (PackedSequences) says which rows are a sequence;
+    a row sees the rows of its own sequence up to itself.  Rows behind the
+    last sequence come back as zeros, and so do their gradients.  Views
+    with any row and head strides are read in place.
+
+    ``bias_table`` [num_buckets, nhead] adds ``relative_position_bias`` of
+    it to the scaled scores without forming the grid; entries of -inf take
+    their distances out, and a row left with nothing is zeros.  ``scale``
+    defaults to d ** -0.5.  What a masked position holds, an infinity or
+    NaN even, does not reach a row that does not see it.
+
+    On the GPU: bfloat16 (fp32 is cast under autocast), d <= 128; sums,
+    softmax statistics and the gradients' sums are fp32, and results do
+    not change from run to run.  The table may be fp32 or bfloat16.
+    """
+    if not isinstance(packing, PackedSequences):
+        raise TypeError("packing has to be a PackedSequences")
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape:
+        raise ValueError(
+            "q is [T, nhead, d], k and v [T, kv_heads, d]: got "
+            f"{tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    rows, nhead, d = q.shape
+    if k.shape[0] != rows or k.shape[2] != d:
+        raise ValueError("q and k differ in rows or head size: "
+                         f"{tuple(q.shape)}, {tuple(k.shape)}")
+    if d < 1 or k.shape[1] < 1 or nhead < 1 or nhead % k.shape[1]:
+        raise ValueError(f"{nhead} heads cannot share {k.shape[1]} "
+                         "key/value heads")
+    if packing.total > rows:
+        raise ValueError(f"the packing has {packing.total} rows, "
+                         f"the tensors {rows}")
+    if len({t.device for t in (q, k, v)}) > 1:
+        raise ValueError("q, k and v are on different devices")
+    if (q.is_cuda and q.dtype == torch.float32
+            and torch.is_autocast_enabled("cuda")):
+        q, k, v = (t.to(torch.bfloat16) for t in (q, k, v))
+    if not (q.is_floating_point() and q.dtype == k.dtype == v.dtype):
+        raise TypeError("q, k and v have to be of one floating type: "
+                        f"{q.dtype}, {k.dtype}, {v.dtype}")
+    scale = d ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < math.inf:
+        raise ValueError(f"scale has to be positive and finite, got {scale}")
+    starts = ()
+    if bias_table is not None:
+        if bias_table.dim() != 2 or bias_table.shape[1] != nhead:
+            raise ValueError(
+                f"the bias table is [num_buckets, {nhead}], got "
+                f"{tuple(bias_table.shape)}")
+        if bias_table.device != q.device:
+            raise ValueError("the bias table is on another device")
+        starts = checked_starts(bias_table.shape[0], max_distance, False)
+    if _use_native("packed_causal_attention", q):
+        if q.dtype != torch.bfloat16 or d > 128:
+            raise TypeError(
+                "packed_causal_attention runs in bfloat16 with a head size "
+                f"of up to 128 on the GPU, got {q.dtype} and {d}")
+        if bias_table is not None and bias_table.dtype not in (
+                torch.bfloat16, torch.float32):
+            raise TypeError("the bias table has to be bfloat16 or float32 "
+                            f"on the GPU, got {bias_table.dtype}")
+        from . import native
+        return native.packed_causal_attention(q, k, v, packing, scale,
+                                              bias_table, starts)
+    return _packed_attention_plain(q, k, v, packing, scale, bias_table,
+                                   max_distance)
+
+
+def _packed_attention_plain(q, k, v, packing, scale, bias_table,
+                            max_distance):
+    wide = torch.promote_types(q.dtype, torch.float32)
+    group = q.shape[1] // k.shape[1]
+    parts = []
+    for first, last in zip(packing.offsets, packing.offsets[1:]):
+        n = last - first
+        qs, ks, vs = (t[first:last].to(wide).transpose(0, 1)
+                      for t in (q, k, v))
+        ks, vs = (t.repeat_interleave(group, 0) for t in (ks, vs))
+        s = torch.matmul(qs, ks.transpose(1, 2)) * scale
+        if bias_table is not None:
+            s = s + relative_position_bias(bias_table.to(wide), n, n,
+                                           max_distance)
+        ahead = torch.ones(n, n, dtype=torch.bool,
+                           device=q.device).triu(1)
+        s = s.masked_fill(ahead, -math.inf)
+        # a row without weight anywhere stays 0 instead of NaN
+        top = s.detach().amax(-1, keepdim=True) if n else s
+        p = torch.exp(s - top.masked_fill(top == -math.inf, 0.0))
+        total = p.sum(-1, keepdim=True)
+        p = p / total.masked_fill(total == 0.0, 1.0)
+        fine = torch.isfinite(vs)
+        out = torch.matmul(p, vs.masked_fill(~fine, 0.0))
+        if not bool(fine.all()):
+            # an infinity or NaN among the values: only rows from there on
+            out = out + vs.masked_fill(fine, 0.0).cumsum(1)
+        parts.append(out.transpose(0, 1).to(q.dtype))
+    rest = q.shape[0] - packing.total
+    parts.append(q.new_zeros(rest, *q.shape[1:]))
+    out = torch.cat(parts)
+    if packing.total == 0:  # gradients of nothing are zeros, not missing
+        for t in (q, k, v, bias_table):
+            if t is not None:
+                out = out + t[:0].sum()
+    return out
 
 
 def avg_pool2d(x, k):

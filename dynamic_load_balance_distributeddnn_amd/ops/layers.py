@@ -85,3 +85,32 @@ class LayerNorm(nn.Module):
     def forward(self, x):
         return FD.layer_norm(x, self.normalized_shape, self.weight, self.bias,
                              self.eps)
+
+
+class RelativePositionBias(nn.Module):
+    """Learned attention bias by bucketed distance, one column a head.
+
+    ``forward`` gives the [nhead, q_len, k_len] grid for attention that
+    takes its bias as a tensor; ``attend`` runs causal attention over
+    packed sequences with the bias added inside the kernel.
+    """
+
+    def __init__(self, nhead, num_buckets=32, max_distance=128,
+                 bidirectional=False):
+        super().__init__()
+        FD.checked_starts(num_buckets, max_distance, bidirectional)
+        self.max_distance, self.bidirectional = max_distance, bidirectional
+        self.weight = nn.Parameter(torch.empty(num_buckets, nhead))
+        nn.init.uniform_(self.weight, -0.1, 0.1)
+
+    def forward(self, q_len, k_len):
+        return FD.relative_position_bias(self.weight, q_len, k_len,
+                                         self.max_distance,
+                                         self.bidirectional)
+
+    def attend(self, q, k, v, packing, scale=None):
+        if self.bidirectional:
+            raise ValueError("packed attention is causal: its bias has one "
+                             "side")
+        return FD.packed_causal_attention(q, k, v, packing, scale,
+                                          self.weight, self.max_distance)

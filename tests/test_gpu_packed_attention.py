@@ -1,0 +1,397 @@
+"""Packed causal attention against its definition in 64 bits."""
+
+import math
+
+import pytest
+import torch
+
+from longctx_reference import attention, check
+
+pytestmark = pytest.mark.gpu
+
+
+def _fd():
+    from dynamic_load_balance_distributeddnn_amd.ops import functional as FD
+    return FD
+
+
+def _inputs(rows, heads, kv, d, seed=0, buckets=0, table_type=torch.float32):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+
+    def normal(*shape, dtype=torch.bfloat16):
+        return torch.randn(*shape, device="cuda", generator=gen).to(dtype)
+
+    q, k, v = normal(rows, heads, d), normal(rows, kv, d), normal(rows, kv, d)
+    do = normal(rows, heads, d)
+    table = normal(buckets, heads, dtype=table_type) if buckets else None
+    return q, k, v, do, table
+
+
+def _run(q, k, v, do, lens, table=None, far=128, scale=None, packing=None):
+    """All outputs by name."""
+    FD = _fd()
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    extra = {}
+    if table is not None:
+        leaves.append(table.detach().requires_grad_())
+        extra = dict(bias_table=leaves[3], max_distance=far)
+    packing = packing or FD.PackedSequences(lens, device=q.device)
+    o = FD.packed_causal_attention(*leaves[:3], packing, scale=scale, **extra)
+    grads = torch.autograd.grad(o, leaves, do)
+    return dict(zip(("o", "dq", "dk", "dv", "dtable"),
+                    (o.detach(), *grads)))
+
+
+def _check_all(got, want, tol, what=""):
+    torch.cuda.synchronize()
+    for name in got:
+        assert got[name].shape == want[name].shape
+        check(got[name], want[name], tol[name], f"{what} {name}")
+
+
+LENGTHS = [[1], [1, 1, 1], [0, 5, 0], [35] * 3, [31, 32, 33], [63, 64, 65],
+           [127, 128, 129], [200, 1, 333], [700]]
+
+
+@pytest.mark.parametrize("lens", LENGTHS, ids=str)
+@pytest.mark.parametrize("heads,kv,d", [(2, 2, 100), (4, 2, 64),
+                                        (8, 1, 128)])
+def test_lengths(lens, heads, kv, d):
+    print(f"lens={lens} heads={heads} kv={kv} d={d}", flush=True)
+    q, k, v, do, _ = _inputs(sum(lens), heads, kv, d)
+    want, tol = attention(q, k, v, lens, do=do)
+    _check_all(_run(q, k, v, do, lens), want, tol)
+
+
+@pytest.mark.parametrize("d", [1, 2, 7, 8, 31, 40, 65, 72, 96, 127])
+def test_head_sizes(d):
+    print(f"d={d}", flush=True)
+    lens = [70, 129]
+    q, k, v, do, _ = _inputs(sum(lens), 3, 3, d, seed=d)
+    want, tol = attention(q, k, v, lens, do=do)
+    _check_all(_run(q, k, v, do, lens), want, tol)
+
+
+@pytest.mark.parametrize("heads,kv", [(1, 1), (6, 3), (16, 8), (24, 8),
+                                      (7, 1)])
+def test_head_layouts(heads, kv):
+    print(f"heads={heads} kv={kv}", flush=True)
+    lens = [150, 33]
+    q, k, v, do, _ = _inputs(sum(lens), heads, kv, 32, seed=heads)
+    want, tol = attention(q, k, v, lens, do=do)
+    _check_all(_run(q, k, v, do, lens), want, tol)
+
+
+@pytest.mark.parametrize("buckets,far,table_type", [
+    (32, 128, torch.float32), (32, 128, torch.bfloat16), (2, 2, torch.float32),
+    (3, 100, torch.float32), (64, 1000, torch.float32),
+    (256, 200, torch.bfloat16)])
+@pytest.mark.parametrize("lens,heads,kv,d", [
+    ([1], 2, 1, 64), ([130, 1, 64], 4, 2, 100), ([600, 300], 2, 2, 128)])
+def test_bias(buckets, far, table_type, lens, heads, kv, d):
+    print(f"{buckets} {far} {table_type} {lens} {heads} {kv} {d}", flush=True)
+    q, k, v, do, table = _inputs(sum(lens), heads, kv, d, buckets=buckets,
+                                 table_type=table_type)
+    want, tol = attention(q, k, v, lens, table=table, far=far, do=do)
+    got = _run(q, k, v, do, lens, table, far)
+    assert got["dtable"].dtype == table_type
+    _check_all(got, want, tol)
+
+
+def test_scale():
+    lens = [90]
+    q, k, v, do, _ = _inputs(90, 2, 2, 64)
+    want, tol = attention(q, k, v, lens, scale=0.3, do=do)
+    _check_all(_run(q, k, v, do, lens, scale=0.3), want, tol)
+
+
+def test_large_scores():
+    """A maximum that grows along the row, far beyond the held one."""
+    lens = [400]
+    q, k, v, do, _ = _inputs(400, 1, 1, 64)
+    grow = torch.linspace(0.1, 3, 400, device="cuda")[:, None, None]
+    k = (k * grow).bfloat16()
+    want, tol = attention(q, k, v, lens, do=do)
+    _check_all(_run(q, k, v, do, lens), want, tol)
+
+
+def test_views_are_read_in_place():
+    """q, k, v as slices of one projection, and heads before rows."""
+    lens = [100, 61]
+    rows, heads, kv, d = 161, 4, 2, 64
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    qkv = torch.randn(rows, (heads + 2 * kv) * d, device="cuda",
+                      generator=gen).bfloat16()
+    q = qkv[:, :heads * d].view(rows, heads, d)
+    k = qkv[:, heads * d:(heads + kv) * d].view(rows, kv, d)
+    v = qkv[:, (heads + kv) * d:].view(rows, kv, d)
+    do = torch.randn(heads, rows, d, device="cuda",
+                     generator=gen).bfloat16().transpose(0, 1)
+    want, tol = attention(q, k, v, lens, do=do)
+    _check_all(_run(q, k, v, do, lens), want, tol)
+
+
+@pytest.mark.parametrize("shift", [1, 2, 4])
+def test_addresses_without_alignment(shift):
+    lens = [100, 40]
+    q, k, v, do, _ = _inputs(140, 2, 1, 64)
+
+    def moved(t):
+        room = torch.zeros(t.numel() + shift, dtype=t.dtype, device="cuda")
+        room[shift:] = t.flatten()
+        return room[shift:].view(t.shape)
+
+    want, tol = attention(q, k, v, lens, do=do)
+    _check_all(_run(moved(q), moved(k), moved(v), moved(do), lens), want, tol)
+
+
+def test_last_dimension_not_dense():
+    lens = [50]
+    q, k, v, do, _ = _inputs(50, 2, 2, 64)
+    want, tol = attention(q, k, v, lens, do=do)
+    turned = [t.transpose(1, 2).contiguous().transpose(1, 2)
+              for t in (q, k, v, do)]
+    _check_all(_run(*turned, lens), want, tol)
+
+
+def test_expanded_gradient():
+    FD = _fd()
+    lens = [77]
+    q, k, v, _, _ = _inputs(77, 2, 2, 64)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    o = FD.packed_causal_attention(*leaves,
+                                   FD.PackedSequences(lens, "cuda"))
+    grads = torch.autograd.grad(o.sum(), leaves)
+    want, tol = attention(q, k, v, lens, do=torch.ones_like(q))
+    _check_all(dict(zip(("dq", "dk", "dv"), grads)), want, tol)
+
+
+def test_rows_behind_the_last_sequence():
+    """Whatever they hold, they come back as zeros and reach nothing."""
+    lens = [100, 30]
+    q, k, v, do, _ = _inputs(150, 4, 2, 64)
+    want, tol = attention(q, k, v, lens, do=do)
+    for t in (q, k, v, do):
+        t[130:] = math.nan
+    got = _run(q, k, v, do, lens)
+    _check_all(got, want, tol)
+    for t in got.values():
+        assert bool((t[130:] == 0).all())
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("at", [5, 70, 129])
+def test_masked_positions_hold_anything(at, value):
+    """Rows before a key or value that is no number do not see it, nor
+    the other sequences."""
+    lens = [40, 150, 45]
+    q, k, v, do, table = _inputs(235, 4, 2, 64, buckets=32)
+    want, tol = attention(q, k, v, lens, do=do, table=table)
+    bad = 40 + at
+    untouched = torch.ones(235, dtype=torch.bool, device="cuda")
+    untouched[bad:190] = False
+    for which in ("k", "v"):
+        kk, vv = k.clone(), v.clone()
+        (kk if which == "k" else vv)[bad] = value
+        got = _run(q, kk, vv, do, lens, table)
+        for name in ("o", "dq"):
+            check(got[name][untouched], want[name][untouched],
+                  tol[name][untouched], f"{which} {name}")
+        if which == "v":
+            assert not torch.isfinite(got["o"][bad:190]).any()
+        else:
+            assert not torch.isfinite(got["o"][bad:190]).all()
+        for name in ("dk", "dv"):
+            other = torch.ones_like(untouched)
+            other[40:190] = False
+            check(got[name][other], want[name][other], tol[name][other],
+                  f"{which} {name}")
+
+
+def test_gradient_of_a_row_reaches_no_key_ahead():
+    lens = [150]
+    q, k, v, do, _ = _inputs(150, 2, 2, 64)
+    want, tol = attention(q, k, v, lens, do=do)
+    for which in ("q", "do"):
+        qq, dd = q.clone(), do.clone()
+        (qq if which == "q" else dd)[70] = math.nan
+        got = _run(qq, k, v, dd, lens)
+        for name in ("dk", "dv"):
+            check(got[name][71:], want[name][71:], tol[name][71:], name)
+        rest = torch.arange(150, device="cuda") != 70
+        check(got["dq"][rest], want["dq"][rest], tol["dq"][rest], "dq")
+
+
+@pytest.mark.parametrize("table_type", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("value", ["lowest", "-inf"])
+@pytest.mark.parametrize("buckets_out", [[5, 6, 7], [31], [0, 1, 2, 3]])
+def test_bias_that_masks(table_type, value, buckets_out):
+    """Distances taken out of a row, up to all of them: zeros with -inf,
+    the mean of equals with the type's lowest value."""
+    lens = [3, 200, 1]
+    q, k, v, do, table = _inputs(204, 2, 2, 64, buckets=32,
+                                 table_type=table_type)
+    low = (torch.finfo(table_type).min if value == "lowest" else -math.inf)
+    table[buckets_out] = low
+    want, tol = attention(q, k, v, lens, do=do, table=table)
+    got = _run(q, k, v, do, lens, table)
+    if value == "lowest":
+        # 64 bits tell scores next to the lowest value apart where fp32
+        # holds the bias alone: rows with nothing else are left to the
+        # bound that no weight depends on
+        if 0 in buckets_out:
+            rows = torch.ones(204, dtype=torch.bool, device="cuda")
+            rows[0:3] = rows[203] = False
+            rows[3:7] = False
+            for name in ("o", "dq"):
+                check(got[name][rows], want[name][rows], tol[name][rows],
+                      name)
+            count = torch.arange(1, 5, device="cuda").double()[:, None, None]
+            mean = v[3:7].double().cumsum(0) / count
+            spread = v[3:7].double().abs().cumsum(0) / count
+            check(got["o"][3:7], mean, 2.1 * 2.0 ** -8 * spread, "mean")
+            assert all(torch.isfinite(t).all() for t in got.values())
+            return
+    _check_all(got, want, tol)
+    if value == "-inf" and 0 in buckets_out:
+        assert bool((got["o"][3:7] == 0).all())
+
+
+def test_same_results_every_time():
+    lens = [300, 513, 2]
+    q, k, v, do, table = _inputs(815, 8, 2, 128, buckets=32)
+    one = _run(q, k, v, do, lens, table)
+    for _ in range(3):
+        two = _run(q, k, v, do, lens, table)
+        for name in one:
+            assert torch.equal(one[name], two[name]), name
+
+
+def test_difference_quotient():
+    """The gradient against differences of the forward in 64 bits: the
+    output moves along a direction as the gradients say."""
+    lens = [60, 21]
+    q, k, v, do, table = _inputs(81, 2, 1, 32, buckets=8)
+    got = _run(q, k, v, do, lens, table, far=20)
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    moves = [torch.randn(t.shape, device="cuda", generator=gen).double()
+             for t in (q, k, v, table)]
+    step = 1e-4
+    ends = []
+    for sign in (1, -1):
+        moved = [t.double() + sign * step * m
+                 for t, m in zip((q, k, v, table), moves)]
+        ends.append(attention(*moved[:3], lens, table=moved[3], far=20)
+                    [0]["o"])
+    slope = ((ends[0] - ends[1]) / (2 * step) * do.double()).sum()
+    names = ("dq", "dk", "dv", "dtable")
+    told = sum((got[n].double() * m).sum() for n, m in zip(names, moves))
+    _, tol = attention(q, k, v, lens, table=table, far=20, do=do)
+    bound = sum((tol[n] * m.abs()).sum() for n, m in zip(names, moves))
+    assert abs(told - slope) <= bound + 1e-4 * abs(slope)
+
+
+def test_side_stream_and_shared_packing():
+    FD = _fd()
+    lens = [100, 290]
+    q, k, v, do, _ = _inputs(390, 4, 4, 64)
+    packing = FD.PackedSequences(lens, device="cuda")
+    want = _run(q, k, v, do, lens, packing=packing)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = _run(q, k, v, do, lens, packing=packing)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    for name in want:
+        assert torch.equal(got[name], want[name]), name
+
+
+def test_captured_and_replayed():
+    """Forward and backward in one graph, replayed on new inputs with
+    eager work in between; two graphs of one packing."""
+    FD = _fd()
+    lens = [100, 64, 170]
+    packing = FD.PackedSequences(lens, device="cuda")
+    sets = [_inputs(334, 4, 2, 64, seed=s, buckets=32) for s in range(4)]
+    graphs = []
+    for g in range(2):
+        static = [t.clone() for t in sets[0]]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            _run(*static[:4], lens, static[4], packing=packing)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = _run(*static[:4], lens, static[4], packing=packing)
+        graphs.append((graph, static, out))
+    for turn in range(4):
+        for g, (graph, static, out) in enumerate(graphs):
+            new = sets[(turn + g) % 4]
+            for s, t in zip(static, new):
+                s.copy_(t)
+            graph.replay()
+            want = _run(*new[:4], lens, new[4], packing=packing)
+            torch.cuda.synchronize()
+            for name in want:
+                assert torch.equal(out[name], want[name]), (turn, g, name)
+
+
+def test_nothing_to_do():
+    FD = _fd()
+    q, k, v, do, table = _inputs(5, 2, 2, 64, buckets=8)
+    got = _run(q, k, v, do, [0, 0], table, far=16)
+    assert all(bool((t == 0).all()) for t in got.values())
+    empty = q[:0]
+    o = FD.packed_causal_attention(empty, empty, empty,
+                                   FD.PackedSequences([], "cuda"))
+    assert o.shape == (0, 2, 64)
+
+
+def test_only_what_is_asked_for():
+    """No gradient for a frozen table, none at all without leaves."""
+    FD = _fd()
+    lens = [140]
+    q, k, v, do, table = _inputs(140, 2, 2, 64, buckets=32)
+    want = _run(q, k, v, do, lens, table)
+    packing = FD.PackedSequences(lens, device="cuda")
+    q.requires_grad_()
+    o = FD.packed_causal_attention(q, k, v, packing, bias_table=table)
+    dq, = torch.autograd.grad(o, q, do)
+    assert torch.equal(dq, want["dq"])
+    with torch.no_grad():
+        o = FD.packed_causal_attention(q, k, v, packing, bias_table=table)
+    assert not o.requires_grad and torch.equal(o, want["o"])
+
+
+def test_refusals_on_the_gpu():
+    FD = _fd()
+    q, k, v, _, table = _inputs(10, 2, 2, 64, buckets=8)
+    packing = FD.PackedSequences([10], device="cuda")
+    with pytest.raises(TypeError):
+        FD.packed_causal_attention(q.float(), k.float(), v.float(), packing)
+    with pytest.raises(TypeError):
+        FD.packed_causal_attention(q.half(), k.half(), v.half(), packing)
+    wide = torch.zeros(10, 2, 136, device="cuda", dtype=torch.bfloat16)
+    with pytest.raises(TypeError):
+        FD.packed_causal_attention(wide, wide, wide, packing)
+    with pytest.raises(TypeError):
+        FD.packed_causal_attention(q, k, v, packing, bias_table=table.half(),
+                                   max_distance=16)
+    with pytest.raises(ValueError):
+        FD.packed_causal_attention(q, k, v, packing, bias_table=table.cpu(),
+                                   max_distance=16)
+    with pytest.raises(TypeError):
+        FD.PackedSequences(torch.tensor([10], device="cuda"))
+
+
+def test_autocast_casts_fp32():
+    FD = _fd()
+    lens = [40]
+    q, k, v, do, _ = _inputs(40, 2, 2, 64)
+    packing = FD.PackedSequences(lens, device="cuda")
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        o = FD.packed_causal_attention(q.float(), k.float(), v.float(),
+                                       packing)
+    assert torch.equal(o, FD.packed_causal_attention(q, k, v, packing))

@@ -1,0 +1,182 @@
+"""Packed causal attention and the position bias on the CPU: the plain
+composition against the definition, and what both refuse."""
+
+import math
+
+import pytest
+import torch
+
+from dynamic_load_balance_distributeddnn_amd.ops import functional as FD
+from dynamic_load_balance_distributeddnn_amd.ops import layers
+from dynamic_load_balance_distributeddnn_amd.ops.packing import (
+    TILE_ROWS, bucket_starts)
+from longctx_reference import attention, bucket_by_count
+
+
+def _inputs(rows, heads, kv, d, buckets=0, dtype=torch.float64):
+    gen = torch.Generator().manual_seed(rows)
+    make = lambda *s: torch.randn(*s, generator=gen, dtype=dtype)  # noqa
+    return (make(rows, heads, d), make(rows, kv, d), make(rows, kv, d),
+            make(rows, heads, d), make(buckets, heads) if buckets else None)
+
+
+@pytest.mark.parametrize("side", [2, 3, 8, 16, 31, 32, 64, 128])
+@pytest.mark.parametrize("far", [128, 200, 1000])
+def test_bucket_starts(side, far):
+    if far <= side // 2:
+        pytest.skip("no distance is left for the logarithm")
+    starts = bucket_starts(side, far)
+    assert len(starts) == side and list(starts) == sorted(starts)
+    edges = torch.tensor(starts)
+    n = torch.arange(far + 50)
+    got = torch.bucketize(n, edges, right=True) - 1
+    want = [bucket_by_count(int(x), side, far) for x in n]
+    assert got.tolist() == want
+
+
+def test_bucket_border_on_a_whole_number():
+    """far / e = 2 ** 4 in 16 steps: every fourth border is a power of 2
+    where a rounded logarithm may fall short of it."""
+    starts = bucket_starts(32, 256)
+    assert [starts[16 + t] for t in (0, 4, 8, 12)] == [16, 32, 64, 128]
+
+
+@pytest.mark.parametrize("lens", [[1], [4, 0, 9], [30], []])
+@pytest.mark.parametrize("heads,kv", [(2, 2), (6, 2)])
+@pytest.mark.parametrize("buckets", [0, 8])
+def test_plain_attention(lens, heads, kv, buckets):
+    rows = sum(lens) + 3
+    q, k, v, do, table = _inputs(rows, heads, kv, 5, buckets)
+    leaves = [t.requires_grad_() for t in (q, k, v, table) if t is not None]
+    o = FD.packed_causal_attention(q, k, v, FD.PackedSequences(lens),
+                                   bias_table=table, max_distance=10)
+    grads = torch.autograd.grad(o, leaves, do, allow_unused=True)
+    if not lens:
+        assert bool((o == 0).all())
+        return
+    want, _ = attention(q, k, v, lens, table=table, far=10, do=do)
+    got = dict(zip(("o", "dq", "dk", "dv", "dtable"), (o, *grads)))
+    for name, value in got.items():
+        torch.testing.assert_close(value, want[name], rtol=1e-9, atol=1e-9)
+
+
+def test_plain_attention_gradcheck():
+    q, k, v, _, table = _inputs(9, 4, 2, 3, 4)
+    pack = FD.PackedSequences([4, 1, 3])
+    leaves = [t.requires_grad_() for t in (q, k, v, table)]
+    assert torch.autograd.gradcheck(
+        lambda q, k, v, t: FD.packed_causal_attention(
+            q, k, v, pack, bias_table=t, max_distance=4), leaves)
+
+
+def test_plain_attention_masked_values():
+    q, k, v, _, table = _inputs(12, 2, 1, 4, 8)
+    pack = FD.PackedSequences([12])
+    want = FD.packed_causal_attention(q, k, v, pack)
+    v2 = v.clone()
+    v2[7] = math.nan
+    got = FD.packed_causal_attention(q, k, v2, pack)
+    torch.testing.assert_close(got[:7], want[:7])
+    assert bool(torch.isnan(got[7:]).all())
+    table[0:2] = -math.inf
+    got = FD.packed_causal_attention(q, k, v, pack, bias_table=table,
+                                     max_distance=16)
+    assert bool((got[:2] == 0).all()) and bool(torch.isfinite(got).all())
+
+
+@pytest.mark.parametrize("both", [False, True])
+def test_plain_bias(both):
+    table = torch.randn(8, 3, dtype=torch.float64, requires_grad=True)
+    out = FD.relative_position_bias(table, 6, 20, 12, both)
+    side = 4 if both else 8
+    for i in range(6):
+        for j in range(20):
+            n = i + 14 - j
+            b = bucket_by_count(abs(n) if both else max(n, 0), side, 12)
+            b += side if both and n < 0 else 0
+            assert torch.equal(out[:, i, j], table[b])
+    assert torch.autograd.gradcheck(
+        lambda t: FD.relative_position_bias(t, 6, 20, 12, both), table)
+
+
+def test_work_lists():
+    """Every row of every sequence in one tile, most work first."""
+    lens = [5, 0, TILE_ROWS, TILE_ROWS + 1, 1000]
+    pack = FD.PackedSequences(torch.tensor(lens))
+    assert pack.total == sum(lens) and len(pack) == 5
+    queries, keys = pack._host_tables()
+    for items in (queries, keys):
+        rows = set()
+        for first, n, tile, _ in items.tolist():
+            assert (first, n) in zip(pack.offsets, lens)
+            top = min(n, (tile + 1) * TILE_ROWS)
+            assert tile * TILE_ROWS < n
+            rows |= {first + r for r in range(tile * TILE_ROWS, top)}
+        assert rows == set(range(sum(lens)))
+        assert len(items) == sum(-(-n // TILE_ROWS) for n in lens)
+    seen = [min(n, (t + 1) * TILE_ROWS) for _, n, t, _ in queries.tolist()]
+    seeing = [n - t * TILE_ROWS for _, n, t, _ in keys.tolist()]
+    assert seen == sorted(seen, reverse=True)
+    assert seeing == sorted(seeing, reverse=True)
+
+
+@pytest.mark.parametrize("lengths,error", [
+    ([3, -1], ValueError), ([2.5], TypeError), ([[1, 2]], TypeError),
+    (torch.tensor([1.0]), TypeError), ([2 ** 30], ValueError),
+    ([True, "x"], TypeError)])
+def test_packing_refusals(lengths, error):
+    with pytest.raises(error):
+        FD.PackedSequences(lengths)
+
+
+def test_attention_refusals():
+    q, k, v, _, table = _inputs(10, 4, 2, 8, 8)
+    pack = FD.PackedSequences([10])
+    call = FD.packed_causal_attention
+    for bad in ((q, k, v, [10]), (q.long(), k.long(), v.long(), pack),
+                (q.float(), k, v, pack)):
+        with pytest.raises(TypeError):
+            call(*bad)
+    for bad in ((q[0], k, v), (q, k, v[:, :1]), (q, k[:9], v[:9]),
+                (q[:, :3], k, v), (q, k[..., :7], v[..., :7]),
+                (q[:9], k[:9], v[:9]), (q[..., :0], k[..., :0], v[..., :0]),
+                (q, k[:, :0], v[:, :0])):
+        with pytest.raises(ValueError):
+            call(*bad, pack)
+    for scale in (0.0, -1.0, math.inf, math.nan):
+        with pytest.raises(ValueError):
+            call(q, k, v, pack, scale=scale)
+    for bad, far in ((table[:, :3], 128), (table[0], 128), (table, 4),
+                     (table[:1], 128), (table, 2 ** 30),
+                     (table.repeat(64, 1), 2000)):
+        with pytest.raises(ValueError):
+            call(q, k, v, pack, bias_table=bad, max_distance=far)
+
+
+def test_bias_refusals():
+    table = torch.zeros(8, 2)
+    call = FD.relative_position_bias
+    for bad in (dict(table=table[0]), dict(q_len=-1), dict(k_len=-1),
+                dict(max_distance=4), dict(table=table[:1]),
+                dict(table=table[:7], bidirectional=True),
+                dict(table=table[:2], bidirectional=True)):
+        args = dict(table=table, q_len=3, k_len=3) | bad
+        with pytest.raises(ValueError):
+            call(**args)
+    with pytest.raises(TypeError):
+        call(table.long(), 3, 3)
+    with pytest.raises(ValueError):
+        layers.RelativePositionBias(2, num_buckets=1)
+
+
+def test_bias_layer():
+    layer = layers.RelativePositionBias(3, 8, 20)
+    assert layer(4, 6).shape == (3, 4, 6)
+    q = torch.randn(6, 3, 4)
+    pack = FD.PackedSequences([6])
+    o = layer.attend(q, q, q, pack)
+    o.sum().backward()
+    assert layer.weight.grad.shape == (8, 3)
+    two_sided = layers.RelativePositionBias(3, 8, 20, bidirectional=True)
+    with pytest.raises(ValueError):
+        two_sided.attend(q, q, q, pack)
