@@ -8,15 +8,24 @@
 //   dK_j = scale sum_i dS_ij q_i          dtable[b] = sum of dS_ij, ij in b
 //
 // Two kernels, each the owner of what it writes: one holds 128 query rows
-// and streams keys (dQ, delta, the table's partial sums), one holds 128
-// keys and streams the queries of every head that shares them (dK, dV).
+// and streams keys (dQ, delta), then one holds 128 keys and streams the
+// queries of every head that shares them (dK, dV, the table's sums).
 // The scores are computed in both, 7 products for 5; in return there are
 // no atomics and no fp32 gradient buffer, and results do not depend on
 // the order in which workgroups run.
+//
+// delta from the stored output carries the output's roundings to bf16
+// (weights, result).  The first kernel sums dS over each row as it goes;
+// the sum is 0 but for that error, so adding it to delta makes delta exact
+// to fp32 for the second kernel: dK and the table's gradient lose nothing
+// to it.  dQ itself is under way by then.  What the error costs it falls
+// with the number of keys that a row's average spreads over, so the first
+// 128 rows of a sequence, which can have few, take delta from a sweep over
+// their one or two key tiles beforehand.
 #include "packed_attn.h"
 
-// Sums of the table's gradient over one 32 x 32 block of dS (keys x
-// queries, the result layout; masked pairs 0): lane l first collects the
+// Sums of the table's gradient over one 32 x 32 block of dS (queries x
+// keys, the result layout; masked pairs 0): lane l first collects the
 // diagonals l & 31 and (l & 31) - 32, then neighbouring diagonals of one
 // bucket are added up lane by lane, in a fixed order.  `n0` is the
 // distance of diagonal 0.  The last bucket is left out: a row's dS sum to
@@ -28,9 +37,9 @@ __device__ inline void pa_bias_sums(const f32x16& ds, int n0,
   float hi = 0.f, lo = 0.f;
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
-    const int from = x + 8 * (r >> 2) + 4 * half + (r & 3);
-    const float v = __shfl(ds[r], (from & 31) + 32 * half, 64);
-    if (from < 32) hi += v; else lo += v;
+    const int i = 8 * (r >> 2) + 4 * half + (r & 3);
+    const float v = __shfl(ds[r], ((i - x) & 31) + 32 * half, 64);
+    if (x <= i) hi += v; else lo += v;
   }
   hi = pa_half_sum(hi);
   lo = pa_half_sum(lo);
@@ -40,9 +49,9 @@ __device__ inline void pa_bias_sums(const f32x16& ds, int n0,
   const int b = n < 0 ? -1 : pa_bucket(starts, buckets, n);
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
-    const int src = (z - off) ^ 32;
-    const float pv = __shfl(v, src & 63, 64);
-    const int pb = __shfl(b, src & 63, 64);
+    const int src = ((z - off) & 63) ^ 32;
+    const float pv = __shfl(v, src, 64);
+    const int pb = __shfl(b, src, 64);
     if (z >= off && pb == b) v += pv;
   }
   const int nb = __shfl(b, ((z + 1) & 63) ^ 32, 64);
@@ -58,13 +67,11 @@ pa_bwd_q_kernel(const PaBwd p, const BiasArg bias) {
   __shared__ float s_win[BIAS ? 2 : 1][BIAS ? 192 : 1];
   __shared__ float s_tab[BIAS ? PA_MAXBUCKETS : 1];
   __shared__ int s_start[BIAS ? PA_MAXBUCKETS : 1];
-  __shared__ float s_hist[BIAS ? 4 : 1][BIAS ? PA_MAXBUCKETS : 1];
 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int col = lane & 31, half = lane >> 5;
   const int h = pa_head(blockIdx.x % p.H, p.H);
-  const int item = blockIdx.x / p.H;
-  const PaItem it = p.items[item];
+  const PaItem it = p.items[blockIdx.x / p.H];
   const int r0 = it.tile * PA_ROWS;
   const int w0 = r0 + wave * 32;
   const int row = w0 + col;
@@ -79,7 +86,6 @@ pa_bwd_q_kernel(const PaBwd p, const BiasArg bias) {
     for (int b = threadIdx.x; b < bias.buckets; b += PA_BLOCK) {
       s_tab[b] = pa_table(bias, b, p.H, h);
       s_start[b] = bias.starts[b];
-      for (int w = 0; w < 4; ++w) s_hist[w][b] = 0.f;
     }
     __syncthreads();
     far_bias = s_tab[bias.buckets - 1];
@@ -95,6 +101,9 @@ pa_bwd_q_kernel(const PaBwd p, const BiasArg bias) {
   };
   auto near = [&](int k0) { return r0 - k0 - (PA_STEP - 1) < far_from; };
 
+  const bool sweep = it.tile == 0;
+  float rest = 0.f;  // this half's sum of the row's dS
+
   bf16x8 qf[KS], gf[KS];
   float delta = 0.f, stat_m = 0.f, stat_l = INFINITY;
   {
@@ -109,9 +118,11 @@ pa_bwd_q_kernel(const PaBwd p, const BiasArg bias) {
       const int dd = VEC ? min(d, p.D - 8) : min(d, p.D - 1);
       qf[s] = pa_load8<VEC>(qb + dd, p.D - d);
       gf[s] = pa_load8<VEC>(gb + dd, p.D - d);
-      const bf16x8 of = pa_load8<VEC>(ob + dd, p.D - d);
+      if (!sweep) {
+        const bf16x8 of = pa_load8<VEC>(ob + dd, p.D - d);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) delta += (float)gf[s][j] * (float)of[j];
+        for (int j = 0; j < 8; ++j) delta += (float)gf[s][j] * (float)of[j];
+      }
     }
     delta = pa_half_sum(delta);
     const long at = (long)h * p.T + rr;
@@ -122,7 +133,6 @@ pa_bwd_q_kernel(const PaBwd p, const BiasArg bias) {
       } else {
         stat_l = p.stats[at];
       }
-      if (half == 0) p.delta[at] = delta;
     }
   }
   const float to2 = BIAS ? PA_LOG2E : p.scale * PA_LOG2E;
@@ -135,20 +145,26 @@ pa_bwd_q_kernel(const PaBwd p, const BiasArg bias) {
   float win = 0.f;
   ks.load(kb, p.k.row, 0, len, p.D);
   vs.load(vb, p.v.row, 0, len, p.D);
-  ks.store(s_k[0]);
-  vs.store(s_v[0]);
+  const int buf0 = sweep ? -tiles & 1 : 0;
+  ks.store(s_k[buf0]);
+  vs.store(s_v[buf0]);
   if constexpr (BIAS) {
-    if (threadIdx.x < 192) s_win[0][threadIdx.x] = window(0);
+    if (threadIdx.x < 192) s_win[buf0][threadIdx.x] = window(0);
   }
   bool bad = __syncthreads_or(PA_STEP > r0 && ks.nonfinite());
 
-  for (int t = 0; t < tiles; ++t) {
-    const int k0 = t * PA_STEP, buf = t & 1;
+  for (int t = sweep ? -tiles : 0; t < tiles; ++t) {
+    if (t == 0 && sweep) {  // with delta 0 the sum of dS was delta
+      delta = pa_half_sum(rest);
+      rest = 0.f;
+    }
+    const int k0 = (t < 0 ? t + tiles : t) * PA_STEP, buf = t & 1;
     const bool more = t + 1 < tiles;
+    const int k1 = t == -1 ? 0 : k0 + PA_STEP;  // of the next tile
     if (more) {
-      ks.load(kb, p.k.row, k0 + PA_STEP, len, p.D);
-      vs.load(vb, p.v.row, k0 + PA_STEP, len, p.D);
-      if (BIAS && near(k0 + PA_STEP)) win = window(k0 + PA_STEP);
+      ks.load(kb, p.k.row, k1, len, p.D);
+      vs.load(vb, p.v.row, k1, len, p.D);
+      if (BIAS && near(k1)) win = window(k1);
     }
     const bool works = k0 <= w0 + 31;
     bf16x8 w[4];
@@ -189,23 +205,20 @@ pa_bwd_q_kernel(const PaBwd p, const BiasArg bias) {
           for (int r = 0; r < 16; ++r)
             if (j * 32 + 8 * (r >> 2) + (r & 3) > lim) s[r] = 0.f;
         }
-        if constexpr (BIAS) {
-          if (w0 - k0 - j * 32 - 31 < far_from && p.part)
-            pa_bias_sums(row < len ? s : pa_zero16(), w0 - k0 - j * 32,
-                         s_start, bias.buckets, s_hist[wave], lane);
-        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) rest += s[r];
         w[2 * j] = pa_operand(s, 0);
         w[2 * j + 1] = pa_operand(s, 1);
       }
     }
-    if (bad) {
+    if (bad && t >= 0) {
       __syncthreads();
       pa_poison<DP, true>(s_k[buf], acc, row - k0, lane);
       __syncthreads();
       pa_cleanse<DP>(s_k[buf]);
       __syncthreads();
     }
-    if (works) {
+    if (works && t >= 0) {
 #pragma unroll
       for (int x = 0; x < 4; ++x)
 #pragma unroll
@@ -216,16 +229,18 @@ pa_bwd_q_kernel(const PaBwd p, const BiasArg bias) {
     if (more) {
       ks.store(s_k[buf ^ 1]);
       vs.store(s_v[buf ^ 1]);
-      if (BIAS && near(k0 + PA_STEP) && threadIdx.x < 192)
+      if (BIAS && near(k1) && threadIdx.x < 192)
         s_win[buf ^ 1][threadIdx.x] = win;
-      if (k0 + 2 * PA_STEP > r0)
+      if (k1 + PA_STEP > r0)
         bad = __syncthreads_or(ks.nonfinite());
       else
         __syncthreads();
     }
   }
 
+  delta += pa_half_sum(rest);
   if (row < len) {
+    if (half == 0) p.delta[(long)h * p.T + it.first + row] = delta;
     __bf16* ob = static_cast<__bf16*>(p.dq) +
                  (((long)it.first + row) * p.H + h) * p.D;
 #pragma unroll
@@ -246,15 +261,6 @@ pa_bwd_q_kernel(const PaBwd p, const BiasArg bias) {
         }
       }
   }
-  if constexpr (BIAS) {
-    if (p.part) {
-      __syncthreads();
-      float* out = p.part + ((long)item * p.H + h) * bias.buckets;
-      for (int b = threadIdx.x; b < bias.buckets; b += PA_BLOCK)
-        out[b] = (s_hist[0][b] + s_hist[1][b]) +
-                 (s_hist[2][b] + s_hist[3][b]);
-    }
-  }
 }
 
 template <int DP, bool VEC, bool BIAS, typename BiasArg>
@@ -268,12 +274,14 @@ pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
   __shared__ __attribute__((aligned(16))) float s_m[2][BIAS ? PA_STEP : 4];
   __shared__ float s_win[BIAS ? 2 : 1][BIAS ? 192 : 1];
   __shared__ int s_start[BIAS ? PA_MAXBUCKETS : 1];
+  __shared__ float s_hist[BIAS ? 4 : 1][BIAS ? PA_MAXBUCKETS : 1];
 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int col = lane & 31, half = lane >> 5;
   const int kvh = p.H / p.G;
   const int hk = pa_head(blockIdx.x % kvh, kvh);
-  const PaItem it = p.items[blockIdx.x / kvh];
+  const long item = blockIdx.x / kvh;
+  const PaItem it = p.items[item];
   const int c0 = it.tile * PA_ROWS;  // first key of the block
   const int w0 = c0 + wave * 32;
   const int key = w0 + col;
@@ -285,8 +293,10 @@ pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
   float far_bias = 0.f;
   int far_from = 0;
   if constexpr (BIAS) {
-    for (int b = threadIdx.x; b < bias.buckets; b += PA_BLOCK)
+    for (int b = threadIdx.x; b < bias.buckets; b += PA_BLOCK) {
       s_start[b] = bias.starts[b];
+      for (int w = 0; w < 4; ++w) s_hist[w][b] = 0.f;
+    }
     far_from = bias.starts[bias.buckets - 1];
   }
   auto near = [&](int q0) { return q0 - c0 - (PA_ROWS - 1) < far_from; };
@@ -428,6 +438,15 @@ pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
           for (int r = 0; r < 16; ++r)
             if (j * 32 + 8 * (r >> 2) + (r & 3) < lim) s[r] = dp[r] = 0.f;
         }
+        if constexpr (BIAS) {
+          const int n0 = q0 + j * 32 - w0;  // of diagonal 0
+          if (p.part && n0 - 31 < far_from) {
+            f32x16 mine = dp;
+            if (key >= len) mine = pa_zero16();
+            pa_bias_sums(mine, n0, s_start, bias.buckets, s_hist[wave],
+                         lane);
+          }
+        }
         pw[2 * j] = pa_operand(s, 0);
         pw[2 * j + 1] = pa_operand(s, 1);
         sw[2 * j] = pa_operand(dp, 0);
@@ -453,6 +472,18 @@ pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
           dk[d] = pa_mfma(pa_col_frag<DP>(s_q[buf], x * 16, d * 32, lane),
                           sw[x], dk[d]);
         }
+    }
+    if constexpr (BIAS) {
+      if (p.part && (step + 1) % nt == 0) {  // a head is done
+        __syncthreads();
+        float* out = p.part +
+                     (item * p.H + hk * p.G + step / nt) * bias.buckets;
+        for (int b = threadIdx.x; b < bias.buckets; b += PA_BLOCK) {
+          out[b] = (s_hist[0][b] + s_hist[1][b]) +
+                   (s_hist[2][b] + s_hist[3][b]);
+          for (int w = 0; w < 4; ++w) s_hist[w][b] = 0.f;
+        }
+      }
     }
     if (more) {
       put(buf ^ 1);
