@@ -20,12 +20,30 @@ struct PaBias {
   int starts[PA_MAXBUCKETS];  // least distance of each bucket
 };
 
-// Work item: one row tile of one sequence.
-struct PaItem {
+// Part of one 128-row tile's work: of a query tile the key tiles (64 keys)
+// begin .. end - 1, of a key tile that many steps (32 queries of a head).
+struct PaChunk {
   int first;  // the sequence's first row
   int len;    // and its rows
-  int tile;   // which tile of 128 rows
-  int pad;
+  int tile;
+  int begin, end;
+  int slot;   // where its sums go, -1: they are the whole tile's
+  int pad[2];
+};
+
+// A tile in several chunks: their slots are slot .. slot + n - 1.
+struct PaJoin {
+  int first, len, tile;
+  int slot, n;
+  int pad[3];
+};
+
+struct PaWork {
+  const PaChunk* chunks;  // most work first
+  const PaJoin* joins;
+  int n_chunks, n_joins;
+  float* sums;   // [slots, heads] of a workgroup's accumulators
+  float* rows;   // [slots, heads, 128, 2] of its row statistics
 };
 
 struct PaFwd {
@@ -33,7 +51,7 @@ struct PaFwd {
   void* o;        // [T, H, D]
   float* stats;   // [H, T]: log2 of the row's sum of exponentials;
                   // with bias [H, T, 2]: maximum, log2 of the sum
-  const PaItem* items;
+  PaWork work;
   int H, G, D;    // heads, heads per key/value head, head size
   long T;
   float scale;
@@ -45,8 +63,8 @@ struct PaBwd {
   const float* stats;  // as the forward left them
   float* delta;        // [H, T]
   void *dq, *dk, *dv;  // [T, H, D], [T, H / G, D] twice
-  float* part;         // [items, H, buckets] of the table's gradient
-  const PaItem* items;
+  float* part;         // [key chunks, H, buckets] of the table's gradient
+  PaWork work_q, work_kv;
   int H, G, D;
   long T;
   float scale;

@@ -6,10 +6,9 @@
 #include "longctx_args.h"
 
 extern "C" void dlb_packed_attn_fwd(const PaFwd* p, const PaBias* bias,
-                                    long items, int vec, hipStream_t stream);
+                                    int width, hipStream_t stream);
 extern "C" void dlb_packed_attn_bwd(const PaBwd* p, const PaBias* bias,
-                                    const PaItem* items_kv, long items,
-                                    int vec, void* dtable, int dtable_bf16,
+                                    int width, void* dtable, int dtable_bf16,
                                     hipStream_t stream);
 extern "C" void dlb_relbias_fwd(const void* table, void* out, const RbArgs* a,
                                 int size, hipStream_t stream);
@@ -42,10 +41,13 @@ static PaTensor pa_tensor(const Tensor& t, const char* name) {
   return {t.data_ptr(), t.stride(0), t.stride(1)};
 }
 
-// 16-byte loads: the head size, the strides and the address allow them.
-static bool pa_vec(const PaTensor& t, int64_t D) {
-  return D % 8 == 0 && t.row % 8 == 0 && t.head % 8 == 0 &&
-         reinterpret_cast<uintptr_t>(t.p) % 16 == 0;
+// Bytes a load may have: the head size, the strides and the address are
+// multiples of them.
+static int pa_width(std::initializer_list<PaTensor> tensors, int64_t D) {
+  int64_t all = D * 2;
+  for (const auto& t : tensors)
+    all |= (t.row | t.head) * 2 | (int64_t)reinterpret_cast<uintptr_t>(t.p);
+  return all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 2;
 }
 
 static void pa_bias(PaBias* b, const Tensor& table, int64_t H,
@@ -65,37 +67,65 @@ static void pa_bias(PaBias* b, const Tensor& table, int64_t H,
 }
 
 static void pa_check(const Tensor& q, const Tensor& k, const Tensor& v,
-                     const Tensor& items, int64_t total) {
+                     int64_t total) {
   TORCH_CHECK(k.sizes() == v.sizes() && q.size(0) == k.size(0) &&
                   q.size(2) == k.size(2) && k.size(1) >= 1 &&
                   q.size(1) % k.size(1) == 0 && q.size(2) >= 1 &&
                   q.size(2) <= 128 && total <= q.size(0) &&
-                  q.size(0) < (1l << 31) / 2,
-              "packed attention: shapes do not fit");
-  TORCH_CHECK(k.device() == q.device() && v.device() == q.device() &&
-                  items.device() == q.device() && items.is_contiguous() &&
-                  items.scalar_type() == torch::kInt32 && items.dim() == 2 &&
-                  items.size(1) == 4 &&
-                  items.size(0) * q.size(1) < (1l << 31),
-              "packed attention: work items do not fit");
+                  q.size(0) < (1l << 31) / 2 && k.device() == q.device() &&
+                  v.device() == q.device(),
+              "packed attention: tensors do not fit");
 }
 
-// q [T, H, D], k and v [T, Hkv, D]; items: the packing's row tiles.  Rows
+// A work list: rows of 8, the chunks, then the joins; `slots` places for
+// the sums of the chunks that are joined, `size` floats for each head's.
+static PaWork pa_work(const Tensor& list, int64_t chunks, int64_t slots,
+                      int64_t heads, int64_t size, const Tensor& like,
+                      std::vector<Tensor>* keep) {
+  TORCH_CHECK(list.device() == like.device() && list.is_contiguous() &&
+                  list.scalar_type() == torch::kInt32 && list.dim() == 2 &&
+                  list.size(1) == 8 && chunks >= 0 &&
+                  chunks <= list.size(0) && slots >= 0 &&
+                  list.size(0) * heads < (1l << 31),
+              "packed attention: work list does not fit");
+  PaWork w{};
+  w.chunks = static_cast<const PaChunk*>(list.data_ptr());
+  w.joins = reinterpret_cast<const PaJoin*>(w.chunks + chunks);
+  w.n_chunks = (int)chunks;
+  w.n_joins = (int)(list.size(0) - chunks);
+  if (slots > 0) {
+    auto sums = torch::empty({slots * heads * (size + 256)},
+                             like.options().dtype(torch::kFloat32));
+    w.sums = sums.data_ptr<float>();
+    w.rows = w.sums + slots * heads * size;
+    keep->push_back(sums);
+  }
+  return w;
+}
+
+// Floats of a workgroup's accumulators, 128 rows of the padded head size.
+static int64_t pa_tile(int64_t D) { return 128 * (D <= 64 ? 64 : 128); }
+
+typedef std::tuple<Tensor, int64_t, int64_t> WorkList;  // chunks, slots
+
+// q [T, H, D], k and v [T, Hkv, D]; work: the packing's query tiles.  Rows
 // from `total` on belong to no sequence and come back as zeros.
 static std::vector<Tensor> packed_attn_fwd(Tensor q, Tensor k, Tensor v,
-                                           Tensor items, int64_t total,
+                                           WorkList work, int64_t total,
                                            double scale, MaybeTensor table,
                                            std::vector<int64_t> starts) {
-  pa_check(q, k, v, items, total);
+  pa_check(q, k, v, total);
   c10::DeviceGuard guard(q.device());
   const int64_t T = q.size(0), H = q.size(1), D = q.size(2);
+  std::vector<Tensor> keep;
   PaFwd p{pa_tensor(q, "q"), pa_tensor(k, "k"), pa_tensor(v, "v")};
   auto o = torch::empty({T, H, D}, q.options());
   auto stats = torch::empty({H, T, table.has_value() ? 2 : 1},
                             q.options().dtype(torch::kFloat32));
   p.o = o.data_ptr();
   p.stats = stats.data_ptr<float>();
-  p.items = static_cast<const PaItem*>(items.data_ptr());
+  p.work = pa_work(std::get<0>(work), std::get<1>(work), std::get<2>(work), H,
+                   pa_tile(D), q, &keep);
   p.H = (int)H;
   p.G = (int)(H / k.size(1));
   p.D = (int)D;
@@ -104,10 +134,9 @@ static std::vector<Tensor> packed_attn_fwd(Tensor q, Tensor k, Tensor v,
   PaBias bias{};
   if (table.has_value()) pa_bias(&bias, *table, H, starts);
   if (total < T) o.slice(0, total).zero_();
-  if (items.size(0) * H > 0) {
-    const bool vec = pa_vec(p.q, D) && pa_vec(p.k, D) && pa_vec(p.v, D);
+  if (p.work.n_chunks > 0) {
     dlb_packed_attn_fwd(&p, table.has_value() ? &bias : nullptr,
-                        items.size(0), vec, current_stream());
+                        pa_width({p.q, p.k, p.v}, D), current_stream());
     launched();
   }
   return {o, stats};
@@ -116,16 +145,16 @@ static std::vector<Tensor> packed_attn_fwd(Tensor q, Tensor k, Tensor v,
 // -> dq, dk, dv and, with a table and `table_grad`, its gradient.
 static std::vector<Tensor> packed_attn_bwd(
     Tensor q, Tensor k, Tensor v, Tensor o, Tensor stats, Tensor go,
-    Tensor items, Tensor items_kv, int64_t total, double scale,
+    WorkList work_q, WorkList work_kv, int64_t total, double scale,
     MaybeTensor table, std::vector<int64_t> starts, bool table_grad) {
-  pa_check(q, k, v, items, total);
-  pa_check(q, k, v, items_kv, total);
+  pa_check(q, k, v, total);
   c10::DeviceGuard guard(q.device());
   const int64_t T = q.size(0), H = q.size(1), D = q.size(2);
-  TORCH_CHECK(go.sizes() == q.sizes() && o.sizes() == q.sizes() &&
-              o.is_contiguous() && stats.is_contiguous() &&
-              stats.numel() == H * T * (table.has_value() ? 2 : 1) &&
-              items.size(0) == items_kv.size(0));
+  TORCH_CHECK(go.sizes() == q.sizes() && go.device() == q.device() &&
+              o.sizes() == q.sizes() && o.is_contiguous() &&
+              stats.is_contiguous() &&
+              stats.numel() == H * T * (table.has_value() ? 2 : 1));
+  std::vector<Tensor> keep;
   PaBwd p{pa_tensor(q, "q"), pa_tensor(k, "k"), pa_tensor(v, "v"),
           pa_tensor(go, "gradient")};
   auto dq = torch::empty({T, H, D}, q.options());
@@ -139,7 +168,11 @@ static std::vector<Tensor> packed_attn_bwd(
   p.dq = dq.data_ptr();
   p.dk = dk.data_ptr();
   p.dv = dv.data_ptr();
-  p.items = static_cast<const PaItem*>(items.data_ptr());
+  p.work_q = pa_work(std::get<0>(work_q), std::get<1>(work_q),
+                     std::get<2>(work_q), H, pa_tile(D), q, &keep);
+  p.work_kv = pa_work(std::get<0>(work_kv), std::get<1>(work_kv),
+                      std::get<2>(work_kv), k.size(1), 2 * pa_tile(D), q,
+                      &keep);
   p.H = (int)H;
   p.G = (int)(H / k.size(1));
   p.D = (int)D;
@@ -151,7 +184,7 @@ static std::vector<Tensor> packed_attn_bwd(
   if (table.has_value()) {
     pa_bias(&bias, *table, H, starts);
     if (table_grad) {
-      part = torch::empty({items.size(0), H, table->size(0)}, f32);
+      part = torch::empty({p.work_kv.n_chunks, H, table->size(0)}, f32);
       dtable = torch::empty_like(*table);
       p.part = part.data_ptr<float>();
       out.push_back(dtable);
@@ -162,16 +195,13 @@ static std::vector<Tensor> packed_attn_bwd(
     dk.slice(0, total).zero_();
     dv.slice(0, total).zero_();
   }
-  if (items.size(0) * H > 0) {
-    const bool vec = pa_vec(p.q, D) && pa_vec(p.k, D) && pa_vec(p.v, D) &&
-                     pa_vec(p.go, D);
+  if (p.work_q.n_chunks > 0) {
     dlb_packed_attn_bwd(&p, table.has_value() ? &bias : nullptr,
-                        static_cast<const PaItem*>(items_kv.data_ptr()),
-                        items.size(0), vec,
-                        table_grad ? dtable.data_ptr() : nullptr,
+                        pa_width({p.q, p.k, p.v, p.go}, D),
+                        dtable.defined() ? dtable.data_ptr() : nullptr,
                         bias.is_bf16, current_stream());
     launched();
-  } else if (table_grad) {
+  } else if (dtable.defined()) {
     dtable.zero_();
   }
   return out;

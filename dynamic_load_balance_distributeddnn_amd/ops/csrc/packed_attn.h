@@ -27,6 +27,7 @@
 #include "longctx_args.h"
 
 #define PA_BLOCK 256
+#define PA_INLINE __attribute__((always_inline))
 #define PA_ROWS 128      // rows of a block's own tile: 4 waves of 32
 #define PA_STEP 64       // rows of a streamed tile
 
@@ -84,24 +85,52 @@ __device__ inline bf16x8 pa_operand(const f32x16& c, int s) {
   return u.v;
 }
 
-// Eight elements from global memory: `left` of them exist (<= 0: none).
-// VEC: 16-byte aligned, and left is <= 0 or >= 8.  The address is clamped
-// by the caller; elements that do not exist are 0.
-template <bool VEC>
-__device__ inline bf16x8 pa_load8(const __bf16* p, int left) {
-  bf16x8 v;
-  if (VEC) {
-    v = *reinterpret_cast<const bf16x8*>(p);
-    u32x4 z = {0u, 0u, 0u, 0u};
-    return left > 0 ? v : __builtin_bit_cast(bf16x8, z);
-  }
+// How a launch moves its tensors: W bytes at a time, 16 where the head
+// size, strides and addresses allow it, else 4, else 2.
+
+// Elements d .. d+7 of a row of D in global memory; those that do not
+// exist are 0.
+template <int W>
+__device__ inline bf16x8 pa_load8(const __bf16* row, int d, int D) {
+  if constexpr (W == 16) {
+    const bf16x8 v = *reinterpret_cast<const bf16x8*>(row + min(d, D - 8));
+    const u32x4 z = {0u, 0u, 0u, 0u};
+    return d < D ? v : __builtin_bit_cast(bf16x8, z);
+  } else if constexpr (W == 4) {
+    u32x4 v;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int jj = j < left ? j : 0;
-    v[j] = p[jj];
-    v[j] = j < left ? v[j] : (__bf16)0.f;
+    for (int j = 0; j < 4; ++j) {
+      const int at = d + 2 * j;
+      const unsigned x =
+          *reinterpret_cast<const unsigned*>(row + min(at, D - 2));
+      v[j] = at < D ? x : 0u;
+    }
+    return __builtin_bit_cast(bf16x8, v);
+  } else {
+    bf16x8 v;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const __bf16 x = row[min(d + j, D - 1)];
+      v[j] = d + j < D ? x : (__bf16)0.f;
+    }
+    return v;
   }
-  return v;
+}
+
+// Elements d .. d+3 of a dense row of D.
+template <int W>
+__device__ inline void pa_store4(__bf16* row, int d, int D, bf16x4 v) {
+  if constexpr (W == 16) {
+    if (d < D) *reinterpret_cast<bf16x4*>(row + d) = v;
+  } else if constexpr (W == 4) {
+    const u32x2 w = __builtin_bit_cast(u32x2, v);
+    if (d < D) *reinterpret_cast<unsigned*>(row + d) = w[0];
+    if (d + 2 < D) *reinterpret_cast<unsigned*>(row + d + 2) = w[1];
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (d + e < D) row[d + e] = v[e];
+  }
 }
 
 // Whether any of eight values is an infinity or a NaN.
@@ -114,83 +143,155 @@ __device__ inline bool pa_nonfinite(bf16x8 v) {
   return bad;
 }
 
-// Operand from the rows of an LDS tile: row `row`, chunk 2*ks + half.
-template <int DP>
-__device__ inline bf16x8 pa_row_frag(const __bf16* tile, int row, int chunk) {
-  return *reinterpret_cast<const bf16x8*>(
-      tile + row * DP + ((chunk ^ pa_swz<DP>(row)) << 3));
-}
-
-// Operand from the columns of an LDS tile: lane l gets column
-// col0 + (l & 31) of the eight rows row0 + 8*(e >> 2) + 4*half + (e & 3).
+// Operands out of LDS tiles.  The swizzle is an exclusive or in bits that
+// a lane's first address and the tiles' bases leave alone, so one address a
+// lane serves all tiles: row operands differ by x << 5, column operands by
+// t << 6, the eight rows further down by 32 and a constant.  fresh() keeps
+// the compiler from holding all of them in registers.
 #define PA_LDS __attribute__((address_space(3)))
 typedef __attribute__((__vector_size__(4 * sizeof(__bf16)))) __bf16 pa_trvec;
+
 template <int DP>
-__device__ inline bf16x8 pa_col_frag(const __bf16* tile, int row0, int col0,
-                                     int lane) {
-  const int r = row0 + 4 * (lane >> 5) + ((lane & 15) >> 2);
-  const int c = (col0 >> 3) + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-  const int in = (lane & 1) * 4;
-  auto p0 = (PA_LDS pa_trvec*)((PA_LDS __bf16*)tile + r * DP +
-                               ((c ^ pa_swz<DP>(r)) << 3) + in);
-  auto p1 = (PA_LDS pa_trvec*)((PA_LDS __bf16*)tile + (r + 8) * DP +
-                               ((c ^ pa_swz<DP>(r + 8)) << 3) + in);
-  union { struct { pa_trvec a, b; } t; bf16x8 v; } u;
-  u.t.a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(p0);
-  u.t.b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(p1);
-  return u.v;
+struct PaFrags {
+  unsigned row;  // chunk `half` of row l & 31
+  unsigned col;  // where lane l starts its transposing reads
+
+  // tiles: 1024-byte aligned
+  __device__ inline explicit PaFrags(const void* tiles, int lane) {
+    const unsigned at = (unsigned)(__UINTPTR_TYPE__)(
+        (PA_LDS const char*)(const char*)tiles);
+    const int r = lane & 31, half = lane >> 5;
+    row = at + r * (DP * 2) + ((half ^ pa_swz<DP>(r)) << 4);
+    const int rc = 4 * half + ((lane & 15) >> 2);
+    const int c = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+    col = at + rc * (DP * 2) + ((c ^ pa_swz<DP>(rc)) << 4) + (lane & 1) * 8;
+  }
+  // The same of tiles `off` bytes on (a multiple of 1024).
+  __device__ PA_INLINE PaFrags fresh(unsigned off = 0) const {
+    PaFrags f = *this;
+    f.row += off;
+    f.col += off;
+    asm volatile("" : "+v"(f.row), "+v"(f.col));
+    return f;
+  }
+  // Row l & 31 of the 32 that start `off` bytes into the tiles, elements
+  // 16 x + 8 half + 0 .. 7.
+  __device__ PA_INLINE bf16x8 rows(unsigned off, int x) const {
+    return *(PA_LDS const bf16x8*)(__UINTPTR_TYPE__)((row ^ (x << 5)) + off);
+  }
+  // Column 32 t + (l & 31) of the 16 rows that start `off` bytes into the
+  // tiles (a multiple of 16 rows), rows 8*(e >> 2) + 4*half + (e & 3).
+  __device__ PA_INLINE bf16x8 cols(unsigned off, int t) const {
+    union { struct { pa_trvec a, b; } t; bf16x8 v; } u;
+    u.t.a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
+        (PA_LDS pa_trvec*)(__UINTPTR_TYPE__)((col ^ (t << 6)) + off));
+    u.t.b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
+        (PA_LDS pa_trvec*)(__UINTPTR_TYPE__)((col ^ (t << 6 | 32)) + off +
+                                             8 * DP * 2));
+    return u.v;
+  }
+};
+
+// W (16 or 4) bytes a lane from base + offset (bytes) to tile + W * lane;
+// base and tile are the wave's.  Written out because the compiler would let
+// every LDS read, of the other buffer too, wait for the load it knows of.
+// Nobody but s_waitcnt vmcnt(0) and a barrier says that the data is there.
+template <int W>
+__device__ inline void pa_to_lds(const __bf16* base, unsigned offset,
+                                 __bf16* tile) {
+  const unsigned to = (unsigned)(__UINTPTR_TYPE__)(
+      (__attribute__((address_space(3))) __bf16*)tile);
+  if constexpr (W == 16)
+    asm volatile(
+        "s_mov_b32 m0, %0\n\ts_nop 0\n\t"
+        "global_load_lds_dwordx4 %1, %2"
+        :: "s"(to), "v"(offset), "s"(base));
+  else
+    asm volatile(
+        "s_mov_b32 m0, %0\n\ts_nop 0\n\t"
+        "global_load_lds_dword %1, %2"
+        :: "s"(to), "v"(offset), "s"(base));
 }
 
-// A streamed [PA_STEP][DP] tile on its way through registers: the next
-// tile's loads are in flight while this one's products run.
-template <int DP, bool VEC>
+// Brings [ROWS][DP] tiles of one sequence's head slice into LDS, the
+// next one while this one's products run: straight from memory, 64 lanes
+// an instruction, the swizzle in the lane's choice of its source.  What is
+// behind D is not loaded: the caller zeroes the buffers once.  Rows behind
+// the sequence repeat its last row; their weights are 0.  W = 2 has no such
+// load and moves its elements in arrive() instead.
+//
+// start() after the barrier that frees the buffer, arrive() before the one
+// that hands it over; both are called by the whole workgroup.
+template <int DP, int W, int ROWS = PA_STEP>
 struct PaStage {
-  static const int CH = DP / 8;
-  static const int N = PA_STEP * CH / PA_BLOCK;
-  bf16x8 v[N];
+  static const int LANES = DP * 2 / W;          // of a row
+  static const int N = ROWS * LANES / PA_BLOCK;
+  const __bf16* base;  // of the sequence's row 0
+  long stride;
+  int len, D;
 
-  // Rows row0 .. of one sequence of `len` rows; `base` its first row's
-  // head slice.  Rows behind the sequence come as zeros.
-  __device__ inline void load(const __bf16* base, long stride, int row0,
-                              int len, int D) {
-    const __bf16* at = base + (long)row0 * stride;
+  template <typename F>
+  __device__ PA_INLINE void each(int row0, F f) {
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int last = len - 1 - row0;  // >= 0: the tile has a row
 #pragma unroll
     for (int u = 0; u < N; ++u) {
-      const int id = threadIdx.x + u * PA_BLOCK;
-      const int r = id / CH, d = (id % CH) * 8;
-      const int rr = min(r, last);
-      const int dd = VEC ? min(d, D - 8) : min(d, D - 1);
-      v[u] = pa_load8<VEC>(at + (unsigned)(rr * (int)stride + dd),
-                           r <= last ? D - d : 0);
+      const int id = (u * (PA_BLOCK / 64) + wave) * 64 + lane;
+      const int r = id / LANES, in = id % LANES * (W / 2);
+      const int col = (((in >> 3) ^ pa_swz<DP>(r)) << 3) + (in & 7);
+      if (col < D)
+        f(id - lane, id, (unsigned)(min(r, last) * (int)stride + col));
     }
   }
-  __device__ inline void store(__bf16* tile) const {
-#pragma unroll
-    for (int u = 0; u < N; ++u) {
-      const int id = threadIdx.x + u * PA_BLOCK;
-      const int r = id / CH, c = id % CH;
-      *reinterpret_cast<bf16x8*>(tile + r * DP +
-                                 ((c ^ pa_swz<DP>(r)) << 3)) = v[u];
+  __device__ PA_INLINE void start(int row0, __bf16* tile) {
+    if constexpr (W > 2) {
+      const __bf16* at = base + (long)row0 * stride;
+      each(row0, [&](int first, int, unsigned from) PA_INLINE {
+        pa_to_lds<W>(at, from * 2, tile + first * (W / 2));
+      });
     }
   }
-  __device__ inline bool nonfinite() const {
-    bool bad = false;
-#pragma unroll
-    for (int u = 0; u < N; ++u) bad |= pa_nonfinite(v[u]);
-    return bad;
+  __device__ PA_INLINE void arrive(int row0, __bf16* tile) {
+    if constexpr (W > 2) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    } else {
+      const __bf16* at = base + (long)row0 * stride;
+      each(row0, [&](int, int id, unsigned from) PA_INLINE {
+        tile[id] = at[from];
+      });
+    }
   }
 };
+
+// Zeroes `rows` rows.
+template <int DP>
+__device__ inline void pa_clear(__bf16* tile, int rows) {
+  const u32x4 z = {0u, 0u, 0u, 0u};
+  for (int i = threadIdx.x; i < rows * DP / 8; i += PA_BLOCK)
+    reinterpret_cast<u32x4*>(tile)[i] = z;
+}
+
+// Whether a tile holds an infinity or NaN (this thread's share of it).
+template <int DP, int ROWS>
+__device__ inline bool pa_tile_nonfinite(const __bf16* tile) {
+  bool bad = false;
+#pragma unroll
+  for (int u = 0; u < ROWS * DP / 8 / PA_BLOCK; ++u)
+    bad |= pa_nonfinite(*reinterpret_cast<const bf16x8*>(
+        tile + (threadIdx.x + u * PA_BLOCK) * 8));
+  return bad;
+}
 
 // A product sums over masked pairs too, with a weight of 0; an infinity
 // or NaN there would come through as NaN.  A tile on the diagonal that
 // holds one is taken apart: acc[column l & 31] += x for each such x of a
 // row that the column may see, and the tile keeps zeros in their place.
 // Columns see row i if i <= lim (DOWN) or i >= lim.
-template <int DP, bool DOWN>
+template <int DP, int ROWS, bool DOWN>
 __device__ inline void pa_poison(const __bf16* tile, f32x16 (&acc)[DP / 32],
                                  int lim, int lane) {
-  for (int i = 0; i < PA_STEP; ++i) {
+  for (int i = 0; i < ROWS; ++i) {
     const bool sees = DOWN ? i <= lim : i >= lim;
 #pragma unroll
     for (int t = 0; t < DP / 32; ++t)
@@ -208,9 +309,9 @@ __device__ inline void pa_poison(const __bf16* tile, f32x16 (&acc)[DP / 32],
       }
   }
 }
-template <int DP>
+template <int DP, int ROWS>
 __device__ inline void pa_cleanse(__bf16* tile) {
-  for (int id = threadIdx.x; id < PA_STEP * DP / 2; id += PA_BLOCK) {
+  for (int id = threadIdx.x; id < ROWS * DP / 2; id += PA_BLOCK) {
     unsigned* w = reinterpret_cast<unsigned*>(tile) + id;
     unsigned x = *w;
     if ((x & 0x7f80u) == 0x7f80u) x &= 0xffff0000u;
@@ -238,6 +339,19 @@ __device__ inline float pa_table(const PaBias& b, int bucket, int heads,
 
 __device__ inline const __bf16* pa_at(const PaTensor& t, long row, int head) {
   return static_cast<const __bf16*>(t.p) + row * t.row + head * t.head;
+}
+
+// Where a workgroup's accumulator `i` (of n, four values a thread) of a
+// chunk goes: consecutive threads next to each other.
+__device__ inline f32x4* pa_sums(const PaWork& w, int slot, int heads, int h,
+                                 int n, int i) {
+  return reinterpret_cast<f32x4*>(w.sums) +
+         (((long)slot * heads + h) * n + i) * PA_BLOCK + threadIdx.x;
+}
+// And its statistics of row `r` of the tile.
+__device__ inline float* pa_rows(const PaWork& w, int slot, int heads, int h,
+                                 int r) {
+  return w.rows + (((long)slot * heads + h) * PA_ROWS + r) * 2;
 }
 
 // Workgroups go round the 8 XCDs in turn.  Where the heads divide, an XCD

@@ -58,27 +58,49 @@ __device__ inline void pa_bias_sums(const f32x16& ds, int n0,
   if (b >= 0 && b < buckets - 1 && (z == 63 || nb != b)) hist[b] += v;
 }
 
-template <int DP, bool VEC, bool BIAS, typename BiasArg>
+// A query row's end: its gradient and delta.
+template <int DP, int W>
+__device__ PA_INLINE void pa_bwd_q_end(const PaBwd& p, long first, int row,
+                                       int len, int h,
+                                       const f32x16 (&acc)[DP / 32],
+                                       float delta) {
+  if (row >= len) return;
+  const int half = (threadIdx.x & 63) >> 5;
+  if (half == 0) p.delta[(long)h * p.T + first + row] = delta;
+  __bf16* ob = static_cast<__bf16*>(p.dq) + ((first + row) * p.H + h) * p.D;
+#pragma unroll
+  for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      bf16x4 v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        v[e] = (__bf16)(acc[t][4 * g + e] * p.scale);
+      pa_store4<W>(ob, t * 32 + 8 * g + 4 * half, p.D, v);
+    }
+}
+
+template <int DP, int W, bool BIAS, typename BiasArg>
 __global__ void __launch_bounds__(PA_BLOCK, 2)
 pa_bwd_q_kernel(const PaBwd p, const BiasArg bias) {
   const int KS = DP / 16, DT = DP / 32;
-  __shared__ __attribute__((aligned(16))) __bf16 s_k[2][PA_STEP * DP];
-  __shared__ __attribute__((aligned(16))) __bf16 s_v[2][PA_STEP * DP];
+  const int TILE = PA_STEP * DP;
+  __shared__ __attribute__((aligned(1024))) __bf16 s_tiles[4][TILE];
+  __bf16 (*s_k)[TILE] = s_tiles, (*s_v)[TILE] = s_tiles + 2;
   __shared__ float s_win[BIAS ? 2 : 1][BIAS ? 192 : 1];
   __shared__ float s_tab[BIAS ? PA_MAXBUCKETS : 1];
   __shared__ int s_start[BIAS ? PA_MAXBUCKETS : 1];
 
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5;
   const int h = pa_head(blockIdx.x % p.H, p.H);
-  const PaItem it = p.items[blockIdx.x / p.H];
+  const PaChunk it = p.work_q.chunks[blockIdx.x / p.H];
   const int r0 = it.tile * PA_ROWS;
   const int w0 = r0 + wave * 32;
   const int row = w0 + col;
   const int len = it.len;
-  const int tiles = (min(r0 + PA_ROWS, len) + PA_STEP - 1) / PA_STEP;
-  const __bf16* kb = pa_at(p.k, it.first, h / p.G);
-  const __bf16* vb = pa_at(p.v, it.first, h / p.G);
+  const int whole = r0 / PA_STEP;  // tiles that all rows see whole
 
   float far_bias = 0.f;
   int far_from = 0;
@@ -91,7 +113,7 @@ pa_bwd_q_kernel(const PaBwd p, const BiasArg bias) {
     far_bias = s_tab[bias.buckets - 1];
     far_from = s_start[bias.buckets - 1];
   }
-  auto window = [&](int k0) {
+  auto window = [&](int k0) PA_INLINE {
     float x = 0.f;
     if constexpr (BIAS) {
       const int n = r0 - k0 - (PA_STEP - 1) + (int)threadIdx.x;
@@ -99,8 +121,11 @@ pa_bwd_q_kernel(const PaBwd p, const BiasArg bias) {
     }
     return x;
   };
-  auto near = [&](int k0) { return r0 - k0 - (PA_STEP - 1) < far_from; };
+  auto near = [&](int k0) PA_INLINE {
+    return r0 - k0 - (PA_STEP - 1) < far_from;
+  };
 
+  // a sequence's first rows, never in chunks: see above
   const bool sweep = it.tile == 0;
   float rest = 0.f;  // this half's sum of the row's dS
 
@@ -115,11 +140,10 @@ pa_bwd_q_kernel(const PaBwd p, const BiasArg bias) {
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       const int d = s * 16 + half * 8;
-      const int dd = VEC ? min(d, p.D - 8) : min(d, p.D - 1);
-      qf[s] = pa_load8<VEC>(qb + dd, p.D - d);
-      gf[s] = pa_load8<VEC>(gb + dd, p.D - d);
+      qf[s] = pa_load8<W>(qb, d, p.D);
+      gf[s] = pa_load8<W>(gb, d, p.D);
       if (!sweep) {
-        const bf16x8 of = pa_load8<VEC>(ob + dd, p.D - d);
+        const bf16x8 of = pa_load8<W>(ob, d, p.D);
 #pragma unroll
         for (int j = 0; j < 8; ++j) delta += (float)gf[s][j] * (float)of[j];
       }
@@ -141,156 +165,226 @@ pa_bwd_q_kernel(const PaBwd p, const BiasArg bias) {
 #pragma unroll
   for (int t = 0; t < DT; ++t) acc[t] = pa_zero16();
 
-  PaStage<DP, VEC> ks, vs;
+  PaStage<DP, W> ks{pa_at(p.k, it.first, h / p.G), p.k.row, len, p.D};
+  PaStage<DP, W> vs{pa_at(p.v, it.first, h / p.G), p.v.row, len, p.D};
   float win = 0.f;
-  ks.load(kb, p.k.row, 0, len, p.D);
-  vs.load(vb, p.v.row, 0, len, p.D);
-  const int buf0 = sweep ? -tiles & 1 : 0;
-  ks.store(s_k[buf0]);
-  vs.store(s_v[buf0]);
-  if constexpr (BIAS) {
-    if (threadIdx.x < 192) s_win[buf0][threadIdx.x] = window(0);
-  }
-  bool bad = __syncthreads_or(PA_STEP > r0 && ks.nonfinite());
+  auto start = [&](int k0, int buf) PA_INLINE {
+    ks.start(k0, s_k[buf]);
+    vs.start(k0, s_v[buf]);
+    if (BIAS && near(k0)) win = window(k0);
+  };
+  auto arrive = [&](int k0, int buf) PA_INLINE {
+    if (BIAS && near(k0) && threadIdx.x < 192) s_win[buf][threadIdx.x] = win;
+    ks.arrive(k0, s_k[buf]);
+    vs.arrive(k0, s_v[buf]);
+    __syncthreads();
+  };
+  const PaFrags<DP> lanes(s_tiles, lane);
+  PaFrags<DP> frags = lanes;  // of the current buffer
+  // weights times (dO.v - delta) of 32 keys of a tile
+  auto gradient = [&](int k0, int j, int buf) PA_INLINE {
+    const unsigned at = j * 32 * DP * 2;
+    f32x16 s = pa_zero16(), dp = pa_zero16();
+#pragma unroll
+    for (int x = 0; x < KS; ++x)
+      s = pa_mfma(frags.rows(at, x), qf[x], s);
+#pragma unroll
+    for (int x = 0; x < KS; ++x)
+      dp = pa_mfma(frags.rows(at + 4 * TILE, x), gf[x], dp);
+    if constexpr (BIAS) {
+      if (near(k0)) {
+        const float* w =
+            s_win[buf] + wave * 32 + col + PA_STEP - 1;
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          s[r] = fmaf(s[r], p.scale,
+                      w[-(j * 32 + 8 * (r >> 2) + 4 * half + (r & 3))]);
+      } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], p.scale, far_bias);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const float e = BIAS ? fmaf(s[r] - stat_m, to2, -stat_l)
+                           : fmaf(s[r], to2, -stat_l);
+      s[r] = __builtin_amdgcn_exp2f(e) * (dp[r] - delta);
+    }
+    return s;
+  };
+  auto product = [&](bf16x8 w, int x) PA_INLINE {
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+      acc[d] = pa_mfma(frags.cols(x * 16 * DP * 2, d), w, acc[d]);
+  };
 
-  for (int t = sweep ? -tiles : 0; t < tiles; ++t) {
-    if (t == 0 && sweep) {  // with delta 0 the sum of dS was delta
-      delta = pa_half_sum(rest);
-      rest = 0.f;
-    }
-    const int k0 = (t < 0 ? t + tiles : t) * PA_STEP, buf = t & 1;
-    const bool more = t + 1 < tiles;
+  // t < 0: the sweep's.
+  auto any_tile = [&](int t) PA_INLINE {
+    const int k0 = (t < 0 ? t + it.end : t) * PA_STEP, buf = t & 1;
     const int k1 = t == -1 ? 0 : k0 + PA_STEP;  // of the next tile
-    if (more) {
-      ks.load(kb, p.k.row, k1, len, p.D);
-      vs.load(vb, p.v.row, k1, len, p.D);
-      if (BIAS && near(k1)) win = window(k1);
-    }
+    if (t + 1 < it.end) start(k1, buf ^ 1);
     const bool works = k0 <= w0 + 31;
     bf16x8 w[4];
+    frags = lanes.fresh(buf * TILE * 2);
     if (works) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        f32x16 s = pa_zero16(), dp = pa_zero16();
-#pragma unroll
-        for (int x = 0; x < KS; ++x) {
-          s = pa_mfma(pa_row_frag<DP>(s_k[buf], j * 32 + col, 2 * x + half),
-                      qf[x], s);
-          dp = pa_mfma(pa_row_frag<DP>(s_v[buf], j * 32 + col, 2 * x + half),
-                       gf[x], dp);
-        }
-        if constexpr (BIAS) {
-          if (near(k0)) {
-            const float* win_at = s_win[buf] + wave * 32 + col + PA_STEP - 1;
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-              s[r] = fmaf(s[r], p.scale,
-                          win_at[-(j * 32 + 8 * (r >> 2) + 4 * half +
-                                   (r & 3))]);
-          } else {
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-              s[r] = fmaf(s[r], p.scale, far_bias);
-          }
-        }
+        f32x16 s = gradient(k0, j, buf);
+        const int lim = row - k0 - 4 * half;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const float e = BIAS ? fmaf(s[r] - stat_m, to2, -stat_l)
-                               : fmaf(s[r], to2, -stat_l);
-          s[r] = __builtin_amdgcn_exp2f(e) * (dp[r] - delta);
+          if (j * 32 + 8 * (r >> 2) + (r & 3) > lim) s[r] = 0.f;
+          rest += s[r];
         }
-        if (k0 + PA_STEP - 1 > w0) {
-          const int lim = row - k0 - 4 * half;
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (j * 32 + 8 * (r >> 2) + (r & 3) > lim) s[r] = 0.f;
-        }
-#pragma unroll
-        for (int r = 0; r < 16; ++r) rest += s[r];
         w[2 * j] = pa_operand(s, 0);
         w[2 * j + 1] = pa_operand(s, 1);
       }
     }
-    if (bad && t >= 0) {
-      __syncthreads();
-      pa_poison<DP, true>(s_k[buf], acc, row - k0, lane);
-      __syncthreads();
-      pa_cleanse<DP>(s_k[buf]);
-      __syncthreads();
-    }
-    if (works && t >= 0) {
-#pragma unroll
-      for (int x = 0; x < 4; ++x)
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-          acc[d] = pa_mfma(pa_col_frag<DP>(s_k[buf], x * 16, d * 32, lane),
-                           w[x], acc[d]);
-    }
-    if (more) {
-      ks.store(s_k[buf ^ 1]);
-      vs.store(s_v[buf ^ 1]);
-      if (BIAS && near(k1) && threadIdx.x < 192)
-        s_win[buf ^ 1][threadIdx.x] = win;
-      if (k1 + PA_STEP > r0)
-        bad = __syncthreads_or(ks.nonfinite());
-      else
+    if (t >= 0) {
+      if (__syncthreads_or(pa_tile_nonfinite<DP, PA_STEP>(s_k[buf]))) {
+        pa_poison<DP, PA_STEP, true>(s_k[buf], acc, row - k0, lane);
         __syncthreads();
+        pa_cleanse<DP, PA_STEP>(s_k[buf]);
+        __syncthreads();
+      }
+      if (works) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) product(w[x], x);
+      }
     }
+    if (t + 1 < it.end) arrive(k1, buf ^ 1);
+  };
+  auto whole_tile = [&](int t) PA_INLINE {
+    const int k0 = t * PA_STEP, buf = t & 1;
+    const bool more = t + 1 < it.end;
+    if (more) start(k0 + PA_STEP, buf ^ 1);
+    frags = lanes.fresh(buf * TILE * 2);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const f32x16 s = gradient(k0, j, buf);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) rest += s[r];
+      product(pa_operand(s, 0), 2 * j);
+      product(pa_operand(s, 1), 2 * j + 1);
+    }
+    if (more) arrive(k0 + PA_STEP, buf ^ 1);
+  };
+
+  if (p.D < DP) {
+    pa_clear<DP>(s_k[0], 2 * PA_STEP);
+    pa_clear<DP>(s_v[0], 2 * PA_STEP);
+    __syncthreads();
+  }
+  int t = sweep ? -it.end : it.begin;
+  start(it.begin * PA_STEP, t & 1);
+  arrive(it.begin * PA_STEP, t & 1);
+  if (!sweep)  // then there are none
+    for (; t < min(whole, it.end); ++t) whole_tile(t);
+  for (; t < it.end; ++t) {
+    if (t == 0 && sweep) {  // with delta 0 the sum of dS was delta
+      delta = pa_half_sum(rest);
+      rest = 0.f;
+    }
+    any_tile(t);
   }
 
-  delta += pa_half_sum(rest);
-  if (row < len) {
-    if (half == 0) p.delta[(long)h * p.T + it.first + row] = delta;
-    __bf16* ob = static_cast<__bf16*>(p.dq) +
-                 (((long)it.first + row) * p.H + h) * p.D;
+  rest = pa_half_sum(rest);
+  if (it.slot >= 0) {
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *pa_sums(p.work_q, it.slot, p.H, h, DT * 4, t * 4 + g) =
+            f32x4{acc[t][4 * g], acc[t][4 * g + 1], acc[t][4 * g + 2],
+                  acc[t][4 * g + 3]};
+    if (half == 0) {
+      float* to = pa_rows(p.work_q, it.slot, p.H, h, wave * 32 + col);
+      to[0] = delta;
+      to[1] = rest;
+    }
+    return;
+  }
+  pa_bwd_q_end<DP, W>(p, it.first, row, len, h, acc, delta + rest);
+}
+
+// Tiles in several chunks: the sums of their sums.
+template <int DP, int W>
+__global__ void __launch_bounds__(PA_BLOCK)
+pa_bwd_q_join_kernel(const PaBwd p) {
+  const int DT = DP / 32;
+  const int h = blockIdx.x % p.H;
+  const PaJoin j = p.work_q.joins[blockIdx.x / p.H];
+  const int in = (threadIdx.x >> 6) * 32 + (threadIdx.x & 31);
+  float delta = pa_rows(p.work_q, j.slot, p.H, h, in)[0];
+  f32x16 acc[DT];
+#pragma unroll
+  for (int t = 0; t < DT; ++t) acc[t] = pa_zero16();
+  for (int i = 0; i < j.n; ++i) {
+    delta += pa_rows(p.work_q, j.slot + i, p.H, h, in)[1];
 #pragma unroll
     for (int t = 0; t < DT; ++t)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const int d = t * 32 + 8 * g + 4 * half;
-        bf16x4 v;
+        const f32x4 x =
+            *pa_sums(p.work_q, j.slot + i, p.H, h, DT * 4, t * 4 + g);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          v[e] = (__bf16)(acc[t][4 * g + e] * p.scale);
-        if (VEC) {
-          if (d < p.D) *reinterpret_cast<bf16x4*>(ob + d) = v;
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (d + e < p.D) ob[d + e] = v[e];
-        }
+        for (int e = 0; e < 4; ++e) acc[t][4 * g + e] += x[e];
       }
   }
+  pa_bwd_q_end<DP, W>(p, j.first, j.tile * PA_ROWS + in, j.len, h, acc,
+                      delta);
 }
 
-template <int DP, bool VEC, bool BIAS, typename BiasArg>
-__global__ void __launch_bounds__(PA_BLOCK, 1)
+// A key row's gradient.
+template <int DP, int W>
+__device__ PA_INLINE void pa_bwd_kv_end(const PaBwd& p, void* out, long row,
+                                        int hk, const f32x16 (&acc)[DP / 32],
+                                        float scale) {
+  const int half = (threadIdx.x & 63) >> 5;
+  __bf16* to = static_cast<__bf16*>(out) + (row * (p.H / p.G) + hk) * p.D;
+#pragma unroll
+  for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      bf16x4 v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = (__bf16)(acc[t][4 * g + e] * scale);
+      pa_store4<W>(to, t * 32 + 8 * g + 4 * half, p.D, v);
+    }
+}
+
+template <int DP, int W, bool BIAS, typename BiasArg>
+__global__ void __launch_bounds__(PA_BLOCK, 2)
 pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
   const int KS = DP / 16, DT = DP / 32;
-  __shared__ __attribute__((aligned(16))) __bf16 s_q[2][PA_STEP * DP];
-  __shared__ __attribute__((aligned(16))) __bf16 s_g[2][PA_STEP * DP];
-  __shared__ __attribute__((aligned(16))) float s_l[2][PA_STEP];
-  __shared__ __attribute__((aligned(16))) float s_delta[2][PA_STEP];
-  __shared__ __attribute__((aligned(16))) float s_m[2][BIAS ? PA_STEP : 4];
+  const int ROWS = 32;  // of a streamed tile
+  const int TILE = ROWS * DP;
+  __shared__ __attribute__((aligned(1024)))
+  __bf16 s_tiles[4 + PA_ROWS / ROWS][TILE];
+  __bf16 (*s_q)[TILE] = s_tiles, (*s_g)[TILE] = s_tiles + 2;
+  __bf16* s_v = s_tiles[4];
+  __shared__ __attribute__((aligned(16))) float s_l[2][ROWS];
+  __shared__ __attribute__((aligned(16))) float s_delta[2][ROWS];
+  __shared__ __attribute__((aligned(16))) float s_m[2][BIAS ? ROWS : 4];
   __shared__ float s_win[BIAS ? 2 : 1][BIAS ? 192 : 1];
   __shared__ int s_start[BIAS ? PA_MAXBUCKETS : 1];
   __shared__ float s_hist[BIAS ? 4 : 1][BIAS ? PA_MAXBUCKETS : 1];
 
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5;
   const int kvh = p.H / p.G;
   const int hk = pa_head(blockIdx.x % kvh, kvh);
-  const long item = blockIdx.x / kvh;
-  const PaItem it = p.items[item];
-  const int c0 = it.tile * PA_ROWS;  // first key of the block
+  const long chunk = blockIdx.x / kvh;
+  const PaChunk it = p.work_kv.chunks[chunk];
+  const int c0 = it.tile * PA_ROWS;  // first key of the workgroup
   const int w0 = c0 + wave * 32;
   const int key = w0 + col;
   const int len = it.len;
-  const int t0 = c0 / PA_STEP;       // first query tile that sees one
-  const int nt = (len + PA_STEP - 1) / PA_STEP - t0;
-  const int steps = nt * p.G;
+  // query tiles from the first that sees a key, for each head
+  const int nt = (len - c0 + ROWS - 1) / ROWS;
 
-  float far_bias = 0.f;
+  float far_bias = 0.f, next_far = 0.f;  // of this and the next step
   int far_from = 0;
   if constexpr (BIAS) {
     for (int b = threadIdx.x; b < bias.buckets; b += PA_BLOCK) {
@@ -298,9 +392,12 @@ pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
       for (int w = 0; w < 4; ++w) s_hist[w][b] = 0.f;
     }
     far_from = bias.starts[bias.buckets - 1];
+    __syncthreads();
   }
-  auto near = [&](int q0) { return q0 - c0 - (PA_ROWS - 1) < far_from; };
-  auto window = [&](int q0, int h) {
+  auto near = [&](int q0) PA_INLINE {
+    return q0 - c0 - (PA_ROWS - 1) < far_from;
+  };
+  auto window = [&](int q0, int h) PA_INLINE {
     float x = 0.f;
     if constexpr (BIAS) {
       const int n = q0 - c0 - (PA_ROWS - 1) + (int)threadIdx.x;
@@ -310,18 +407,12 @@ pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
     return x;
   };
 
-  bf16x8 kf[KS], vf[KS];
+  bf16x8 kf[KS];
   {
-    const long rr = (long)it.first + min(key, len - 1);
-    const __bf16* kb = pa_at(p.k, rr, hk);
-    const __bf16* vb = pa_at(p.v, rr, hk);
+    const __bf16* kb = pa_at(p.k, (long)it.first + min(key, len - 1), hk);
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      const int d = s * 16 + half * 8;
-      const int dd = VEC ? min(d, p.D - 8) : min(d, p.D - 1);
-      kf[s] = pa_load8<VEC>(kb + dd, p.D - d);
-      vf[s] = pa_load8<VEC>(vb + dd, p.D - d);
-    }
+    for (int s = 0; s < KS; ++s)
+      kf[s] = pa_load8<W>(kb, s * 16 + half * 8, p.D);
   }
   const float to2 = BIAS ? PA_LOG2E : p.scale * PA_LOG2E;
 
@@ -329,14 +420,15 @@ pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
 #pragma unroll
   for (int t = 0; t < DT; ++t) dk[t] = dv[t] = pa_zero16();
 
-  PaStage<DP, VEC> qs, gs;
+  PaStage<DP, W, ROWS> qs{nullptr, p.q.row, len, p.D};
+  PaStage<DP, W, ROWS> gs{nullptr, p.go.row, len, p.D};
   float win = 0.f, st_l = 0.f, st_d = 0.f, st_m = 0.f;
-  auto fetch = [&](int step) {
-    const int h = hk * p.G + step / nt;
-    const int q0 = (t0 + step % nt) * PA_STEP;
-    qs.load(pa_at(p.q, it.first, h), p.q.row, q0, len, p.D);
-    gs.load(pa_at(p.go, it.first, h), p.go.row, q0, len, p.D);
-    if (threadIdx.x < PA_STEP) {
+  auto start = [&](int q0, int h, int buf) PA_INLINE {
+    qs.base = pa_at(p.q, it.first, h);
+    gs.base = pa_at(p.go, it.first, h);
+    qs.start(q0, s_q[buf]);
+    gs.start(q0, s_g[buf]);
+    if (threadIdx.x < ROWS) {
       // rows behind the sequence: weights of exp2(-inf)
       st_l = INFINITY;
       st_d = st_m = 0.f;
@@ -352,191 +444,264 @@ pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
         st_d = p.delta[at];
       }
     }
-    if (BIAS) {
-      if (near(q0)) win = window(q0, h);
-      else win = 0.f;
-    }
+    if (BIAS && near(q0)) win = window(q0, h);
+    if constexpr (BIAS) next_far = pa_table(bias, bias.buckets - 1, p.H, h);
   };
-  auto put = [&](int buf) {
-    qs.store(s_q[buf]);
-    gs.store(s_g[buf]);
-    if (threadIdx.x < PA_STEP) {
+  auto arrive = [&](int q0, int buf) PA_INLINE {
+    if (threadIdx.x < ROWS) {
       s_l[buf][threadIdx.x] = st_l;
       s_delta[buf][threadIdx.x] = st_d;
       if (BIAS) s_m[buf][threadIdx.x] = st_m;
     }
-    if (BIAS && threadIdx.x < 192) s_win[buf][threadIdx.x] = win;
-  };
-  auto diagonal = [&](int step) {
-    return (t0 + step % nt) * PA_STEP < c0 + PA_ROWS;
+    if (BIAS && near(q0) && threadIdx.x < 192) s_win[buf][threadIdx.x] = win;
+    far_bias = next_far;
+    qs.arrive(q0, s_q[buf]);
+    gs.arrive(q0, s_g[buf]);
+    __syncthreads();
   };
 
-  if (BIAS) __syncthreads();
-  fetch(0);
-  put(0);
-  bool bad = __syncthreads_or(qs.nonfinite() || gs.nonfinite());
-  int head_now = -1;
+  const PaFrags<DP> lanes(s_tiles, lane);
+  PaFrags<DP> frags = lanes;  // of the current buffer
+  // s: the weights, dp: their gradient, of 32 queries of a tile
+  auto gradient = [&](f32x16& s, f32x16& dp, int q0,
+                      int buf) PA_INLINE {
+    const PaFrags<DP> vfrags = lanes.fresh(wave * (32 * DP * 2));
+    s = dp = pa_zero16();
+#pragma unroll
+    for (int x = 0; x < KS; ++x)
+      s = pa_mfma(frags.rows(0, x), kf[x], s);
+#pragma unroll
+    for (int x = 0; x < KS; ++x)
+      dp = pa_mfma(frags.rows(2 * TILE * 2, x),
+                   vfrags.rows(4 * TILE * 2, x), dp);
+    if constexpr (BIAS) {
+      if (near(q0)) {
+        const float* w = s_win[buf] + PA_ROWS - 1 - wave * 32 - col;
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          s[r] = fmaf(s[r], p.scale,
+                      w[8 * (r >> 2) + 4 * half + (r & 3)]);
+      } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], p.scale, far_bias);
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int at = 8 * g + 4 * half;
+      const f32x4 lv = *reinterpret_cast<const f32x4*>(&s_l[buf][at]);
+      const f32x4 ev = *reinterpret_cast<const f32x4*>(&s_delta[buf][at]);
+      f32x4 mv = {0.f, 0.f, 0.f, 0.f};
+      if constexpr (BIAS)
+        mv = *reinterpret_cast<const f32x4*>(&s_m[buf][at]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = 4 * g + e;
+        s[r] = __builtin_amdgcn_exp2f(BIAS
+                                          ? fmaf(s[r] - mv[e], to2, -lv[e])
+                                          : fmaf(s[r], to2, -lv[e]));
+        dp[r] = s[r] * (dp[r] - ev[e]);
+      }
+    }
+  };
+  auto table_sums = [&](const f32x16& dp, int q0) PA_INLINE {
+    if constexpr (BIAS) {
+      const int n0 = q0 - w0;  // distance of diagonal 0
+      if (p.part && n0 - 31 < far_from) {
+        f32x16 mine = dp;
+        if (key >= len) mine = pa_zero16();
+        pa_bias_sums(mine, n0, s_start, bias.buckets, s_hist[wave], lane);
+      }
+    }
+  };
+  auto product = [&](bf16x8 pw, bf16x8 sw, int x) PA_INLINE {
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+      dv[d] = pa_mfma(
+          frags.cols((2 * ROWS + x * 16) * DP * 2, d), pw, dv[d]);
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+      dk[d] = pa_mfma(frags.cols(x * 16 * DP * 2, d), sw, dk[d]);
+  };
 
-  for (int step = 0; step < steps; ++step) {
+  // Step `step`: query tile q0 of a head; q1 and h1 are the next step's.
+  auto any_tile = [&](int step, int q0, int q1, int h1) PA_INLINE {
     const int buf = step & 1;
-    const int q0 = (t0 + step % nt) * PA_STEP;
-    const bool more = step + 1 < steps;
-    if (more) fetch(step + 1);
-    if constexpr (BIAS) {
-      const int h = hk * p.G + step / nt;
-      if (h != head_now) {
-        head_now = h;
-        far_bias = pa_table(bias, bias.buckets - 1, p.H, h);
-      }
-    }
-    const bool works = q0 + PA_STEP - 1 >= w0;
-    bf16x8 pw[4], sw[4];
+    const bool more = step + 1 < it.end;
+    if (more) start(q1, h1, buf ^ 1);
+    const bool works = q0 + ROWS - 1 >= w0;
+    frags = lanes.fresh(buf * TILE * 2);
+    f32x16 s, dp;
     if (works) {
+      gradient(s, dp, q0, buf);
+      const int lim = key - q0 - 4 * half;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        f32x16 s = pa_zero16(), dp = pa_zero16();
-#pragma unroll
-        for (int x = 0; x < KS; ++x) {
-          s = pa_mfma(pa_row_frag<DP>(s_q[buf], j * 32 + col, 2 * x + half),
-                      kf[x], s);
-          dp = pa_mfma(pa_row_frag<DP>(s_g[buf], j * 32 + col, 2 * x + half),
-                       vf[x], dp);
-        }
-        if constexpr (BIAS) {
-          if (near(q0)) {
-            const float* win_at = s_win[buf] + PA_ROWS - 1 - wave * 32 - col;
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-              s[r] = fmaf(s[r], p.scale,
-                          win_at[j * 32 + 8 * (r >> 2) + 4 * half + (r & 3)]);
-          } else {
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-              s[r] = fmaf(s[r], p.scale, far_bias);
-          }
-        }
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const int at = j * 32 + 8 * g + 4 * half;
-          const f32x4 lv = *reinterpret_cast<const f32x4*>(&s_l[buf][at]);
-          const f32x4 ev = *reinterpret_cast<const f32x4*>(&s_delta[buf][at]);
-          f32x4 mv = {0.f, 0.f, 0.f, 0.f};
-          if constexpr (BIAS)
-            mv = *reinterpret_cast<const f32x4*>(&s_m[buf][at]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int r = 4 * g + e;
-            s[r] = __builtin_amdgcn_exp2f(
-                BIAS ? fmaf(s[r] - mv[e], to2, -lv[e])
-                     : fmaf(s[r], to2, -lv[e]));
-            dp[r] = s[r] * (dp[r] - ev[e]);
-          }
-        }
-        if (q0 < w0 + 31) {
-          const int lim = key - q0 - 4 * half;
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (j * 32 + 8 * (r >> 2) + (r & 3) < lim) s[r] = dp[r] = 0.f;
-        }
-        if constexpr (BIAS) {
-          const int n0 = q0 + j * 32 - w0;  // of diagonal 0
-          if (p.part && n0 - 31 < far_from) {
-            f32x16 mine = dp;
-            if (key >= len) mine = pa_zero16();
-            pa_bias_sums(mine, n0, s_start, bias.buckets, s_hist[wave],
-                         lane);
-          }
-        }
-        pw[2 * j] = pa_operand(s, 0);
-        pw[2 * j + 1] = pa_operand(s, 1);
-        sw[2 * j] = pa_operand(dp, 0);
-        sw[2 * j + 1] = pa_operand(dp, 1);
-      }
+      for (int r = 0; r < 16; ++r)
+        if (8 * (r >> 2) + (r & 3) < lim) s[r] = dp[r] = 0.f;
+      table_sums(dp, q0);
     }
-    if (bad) {
+    if (__syncthreads_or(pa_tile_nonfinite<DP, ROWS>(s_q[buf]) ||
+                         pa_tile_nonfinite<DP, ROWS>(s_g[buf]))) {
+      pa_poison<DP, ROWS, false>(s_g[buf], dv, key - q0, lane);
+      pa_poison<DP, ROWS, false>(s_q[buf], dk, key - q0, lane);
       __syncthreads();
-      pa_poison<DP, false>(s_g[buf], dv, key - q0, lane);
-      pa_poison<DP, false>(s_q[buf], dk, key - q0, lane);
-      __syncthreads();
-      pa_cleanse<DP>(s_g[buf]);
-      pa_cleanse<DP>(s_q[buf]);
+      pa_cleanse<DP, ROWS>(s_g[buf]);
+      pa_cleanse<DP, ROWS>(s_q[buf]);
       __syncthreads();
     }
     if (works) {
-#pragma unroll
-      for (int x = 0; x < 4; ++x)
-#pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          dv[d] = pa_mfma(pa_col_frag<DP>(s_g[buf], x * 16, d * 32, lane),
-                          pw[x], dv[d]);
-          dk[d] = pa_mfma(pa_col_frag<DP>(s_q[buf], x * 16, d * 32, lane),
-                          sw[x], dk[d]);
-        }
+      product(pa_operand(s, 0), pa_operand(dp, 0), 0);
+      product(pa_operand(s, 1), pa_operand(dp, 1), 1);
     }
+    if (more) arrive(q1, buf ^ 1);
+  };
+  auto whole_tile = [&](int step, int q0, int q1, int h1) PA_INLINE {
+    const int buf = step & 1;
+    const bool more = step + 1 < it.end;
+    if (more) start(q1, h1, buf ^ 1);
+    frags = lanes.fresh(buf * TILE * 2);
+    f32x16 s, dp;
+    gradient(s, dp, q0, buf);
+    table_sums(dp, q0);
+    product(pa_operand(s, 0), pa_operand(dp, 0), 0);
+    product(pa_operand(s, 1), pa_operand(dp, 1), 1);
+    if (more) arrive(q1, buf ^ 1);
+  };
+
+  if (p.D < DP) {
+    pa_clear<DP>(s_q[0], 2 * ROWS);
+    pa_clear<DP>(s_g[0], 2 * ROWS);
+    pa_clear<DP>(s_v, PA_ROWS);
+    __syncthreads();
+  }
+  {
+    PaStage<DP, W, ROWS> vs{pa_at(p.v, it.first, hk), p.v.row, len, p.D};
+    for (int r = 0; r < PA_ROWS && c0 + r < len; r += ROWS) {
+      vs.start(c0 + r, s_v + r * DP);
+      vs.arrive(c0 + r, s_v + r * DP);
+    }
+  }
+  // The order of the steps: first the tiles that need neither a mask nor
+  // the table's sums, from the sequence's end backwards and every head of
+  // a tile in turn, so that the workgroups of a sequence read the same
+  // queries at the same time, from L2; then the others, head by head.
+  int other = min(PA_ROWS / ROWS, nt);  // tiles of the second part
+  if (BIAS && p.part)
+    other = min(max(other, (far_from + PA_ROWS + ROWS - 1) / ROWS), nt);
+  const int h0 = hk * p.G, bulk = (nt - other) * p.G;
+  // tile and head of a step
+  auto tile_of = [&](int s) PA_INLINE {
+    return s < bulk ? nt - 1 - s / p.G : other - 1 - (s - bulk) % other;
+  };
+  auto head_of = [&](int s) PA_INLINE {
+    return s < bulk ? s % p.G : (s - bulk) / other;
+  };
+  int step = it.begin, t = tile_of(step), g = head_of(step);
+  start(c0 + t * ROWS, h0 + g, step & 1);
+  arrive(c0 + t * ROWS, step & 1);
+  auto go = [&](auto tile) PA_INLINE {
+    const int q0 = c0 + t * ROWS;
+    const bool last = step + 1 < bulk ? g + 1 == p.G : t == 0;
+    if (step + 1 < bulk) {
+      t -= last;
+      g = last ? 0 : g + 1;
+    } else if (step + 1 == bulk) {
+      t = other - 1;
+      g = 0;
+    } else {
+      g += last;
+      t = last ? other - 1 : t - 1;
+    }
+    tile(step++, q0, c0 + t * ROWS, h0 + g);
+  };
+  while (step < min(bulk, it.end)) go(whole_tile);
+  const int g_first = g;
+  while (step < it.end) {
+    const int head = g;
+    const int stop = min(bulk + (head + 1) * other, it.end);
+    while (t >= PA_ROWS / ROWS && step < stop) go(whole_tile);
+    while (step < stop) go(any_tile);
     if constexpr (BIAS) {
-      if (p.part && (step + 1) % nt == 0) {  // a head is done
+      if (p.part) {
         __syncthreads();
-        float* out = p.part +
-                     (item * p.H + hk * p.G + step / nt) * bias.buckets;
+        float* out = p.part + (chunk * p.H + h0 + head) * bias.buckets;
         for (int b = threadIdx.x; b < bias.buckets; b += PA_BLOCK) {
           out[b] = (s_hist[0][b] + s_hist[1][b]) +
                    (s_hist[2][b] + s_hist[3][b]);
           for (int w = 0; w < 4; ++w) s_hist[w][b] = 0.f;
         }
-      }
-    }
-    if (more) {
-      put(buf ^ 1);
-      if (diagonal(step + 1))
-        bad = __syncthreads_or(qs.nonfinite() || gs.nonfinite());
-      else {
-        bad = false;
         __syncthreads();
       }
     }
   }
-
-  if (key >= len) return;
-  const long at = (((long)it.first + key) * kvh + hk) * p.D;
-  __bf16* okb = static_cast<__bf16*>(p.dk) + at;
-  __bf16* ovb = static_cast<__bf16*>(p.dv) + at;
-#pragma unroll
-  for (int t = 0; t < DT; ++t)
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int d = t * 32 + 8 * g + 4 * half;
-      bf16x4 a, b;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        a[e] = (__bf16)(dk[t][4 * g + e] * p.scale);
-        b[e] = (__bf16)dv[t][4 * g + e];
-      }
-      if (VEC) {
-        if (d < p.D) {
-          *reinterpret_cast<bf16x4*>(okb + d) = a;
-          *reinterpret_cast<bf16x4*>(ovb + d) = b;
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (d + e < p.D) {
-            okb[d + e] = a[e];
-            ovb[d + e] = b[e];
-          }
-      }
+  if constexpr (BIAS) {
+    if (p.part) {  // heads that only other chunks have sums for
+      const int g_end = it.end > bulk ? (it.end - 1 - bulk) / other : -1;
+      for (int x = 0; x < p.G; ++x)
+        if (it.end <= bulk || x < g_first || x > g_end)
+          for (int b = threadIdx.x; b < bias.buckets; b += PA_BLOCK)
+            p.part[(chunk * p.H + h0 + x) * bias.buckets + b] = 0.f;
     }
+  }
+
+  if (it.slot >= 0) {
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        *pa_sums(p.work_kv, it.slot, kvh, hk, DT * 8, t * 8 + g) =
+            f32x4{dk[t][4 * g], dk[t][4 * g + 1], dk[t][4 * g + 2],
+                  dk[t][4 * g + 3]};
+        *pa_sums(p.work_kv, it.slot, kvh, hk, DT * 8, t * 8 + 4 + g) =
+            f32x4{dv[t][4 * g], dv[t][4 * g + 1], dv[t][4 * g + 2],
+                  dv[t][4 * g + 3]};
+      }
+    return;
+  }
+  if (key < len) {
+    const long at = (long)it.first + key;
+    pa_bwd_kv_end<DP, W>(p, p.dk, at, hk, dk, p.scale);
+    pa_bwd_kv_end<DP, W>(p, p.dv, at, hk, dv, 1.f);
+  }
 }
 
-// dtable[b, h] from the items' partial sums; a workgroup a head, a wave a
+// Tiles in several chunks: the sums of their sums; blockIdx.y: dK or dV.
+template <int DP, int W>
+__global__ void __launch_bounds__(PA_BLOCK)
+pa_bwd_kv_join_kernel(const PaBwd p) {
+  const int DT = DP / 32;
+  const int kvh = p.H / p.G, hk = blockIdx.x % kvh;
+  const PaJoin j = p.work_kv.joins[blockIdx.x / kvh];
+  const int key = j.tile * PA_ROWS + (threadIdx.x >> 6) * 32 +
+                  (threadIdx.x & 31);
+  f32x16 acc[DT];
+#pragma unroll
+  for (int t = 0; t < DT; ++t) acc[t] = pa_zero16();
+  for (int i = 0; i < j.n; ++i)
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 x = *pa_sums(p.work_kv, j.slot + i, kvh, hk, DT * 8,
+                                 t * 8 + 4 * (int)blockIdx.y + g);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[t][4 * g + e] += x[e];
+      }
+  if (key < j.len)
+    pa_bwd_kv_end<DP, W>(p, blockIdx.y ? p.dv : p.dk, (long)j.first + key, hk,
+                         acc, blockIdx.y ? 1.f : p.scale);
+}
+
+// dtable[b, h] from the chunks' partial sums; a workgroup a head, a wave a
 // bucket at a time, every sum in a fixed order.
 __global__ void __launch_bounds__(PA_BLOCK)
 pa_table_grad_kernel(const float* __restrict__ part, void* out, int is_bf16,
-                     long items, int H, int buckets) {
+                     long chunks, int H, int buckets) {
   __shared__ float s_sum[PA_MAXBUCKETS];
   const int h = blockIdx.x, lane = threadIdx.x & 63;
   for (int b = threadIdx.x >> 6; b < buckets - 1; b += PA_BLOCK / 64) {
     float v = 0.f;
-    for (long i = lane; i < items; i += 64)
+    for (long i = lane; i < chunks; i += 64)
       v += part[(i * H + h) * buckets + b];
     v = wave_reduce_sum(v);
     if (lane == 0) s_sum[b] = v;
@@ -557,40 +722,46 @@ pa_table_grad_kernel(const float* __restrict__ part, void* out, int is_bf16,
   }
 }
 
-template <int DP, bool VEC>
-static void pa_bwd_go(const PaBwd& p, const PaBwd& pk, const PaBias* bias,
-                      unsigned grid, unsigned grid_kv, hipStream_t stream) {
-  if (bias) {
-    hipLaunchKernelGGL((pa_bwd_q_kernel<DP, VEC, true, PaBias>), dim3(grid),
-                       dim3(PA_BLOCK), 0, stream, p, *bias);
-    hipLaunchKernelGGL((pa_bwd_kv_kernel<DP, VEC, true, PaBias>),
-                       dim3(grid_kv), dim3(PA_BLOCK), 0, stream, pk, *bias);
-  } else {
-    hipLaunchKernelGGL((pa_bwd_q_kernel<DP, VEC, false, PaNoBias>),
-                       dim3(grid), dim3(PA_BLOCK), 0, stream, p, PaNoBias{});
-    hipLaunchKernelGGL((pa_bwd_kv_kernel<DP, VEC, false, PaNoBias>),
-                       dim3(grid_kv), dim3(PA_BLOCK), 0, stream, pk,
-                       PaNoBias{});
-  }
+template <int DP, int W>
+static void pa_bwd_go(const PaBwd& p, const PaBias* bias,
+                      hipStream_t stream) {
+  const unsigned H = p.H, kvh = p.H / p.G;
+  const dim3 block(PA_BLOCK);
+  const dim3 grid(p.work_q.n_chunks * H), joins(p.work_q.n_joins * H);
+  const dim3 grid_kv(p.work_kv.n_chunks * kvh);
+  const dim3 joins_kv(p.work_kv.n_joins * kvh, 2);
+  if (bias)
+    hipLaunchKernelGGL((pa_bwd_q_kernel<DP, W, true, PaBias>), grid, block, 0,
+                       stream, p, *bias);
+  else
+    hipLaunchKernelGGL((pa_bwd_q_kernel<DP, W, false, PaNoBias>), grid, block,
+                       0, stream, p, PaNoBias{});
+  if (joins.x)
+    hipLaunchKernelGGL((pa_bwd_q_join_kernel<DP, W>), joins, block, 0, stream,
+                       p);
+  if (bias)
+    hipLaunchKernelGGL((pa_bwd_kv_kernel<DP, W, true, PaBias>), grid_kv,
+                       block, 0, stream, p, *bias);
+  else
+    hipLaunchKernelGGL((pa_bwd_kv_kernel<DP, W, false, PaNoBias>), grid_kv,
+                       block, 0, stream, p, PaNoBias{});
+  if (joins_kv.x)
+    hipLaunchKernelGGL((pa_bwd_kv_join_kernel<DP, W>), joins_kv, block, 0,
+                       stream, p);
 }
 
-// `items_kv`: the same tiles as keys, longest remainder first.
+// width: as in the forward.
 extern "C" void dlb_packed_attn_bwd(const PaBwd* p, const PaBias* bias,
-                                    const PaItem* items_kv, long items,
-                                    int vec, void* dtable, int dtable_bf16,
+                                    int width, void* dtable, int dtable_bf16,
                                     hipStream_t stream) {
-  PaBwd pk = *p;
-  pk.items = items_kv;
-  const unsigned grid = (unsigned)(items * p->H);
-  const unsigned grid_kv = (unsigned)(items * (p->H / p->G));
-  if (p->D <= 64)
-    vec ? pa_bwd_go<64, true>(*p, pk, bias, grid, grid_kv, stream)
-        : pa_bwd_go<64, false>(*p, pk, bias, grid, grid_kv, stream);
-  else
-    vec ? pa_bwd_go<128, true>(*p, pk, bias, grid, grid_kv, stream)
-        : pa_bwd_go<128, false>(*p, pk, bias, grid, grid_kv, stream);
+  auto go = [&](auto go64, auto go128) {
+    (p->D <= 64 ? go64 : go128)(*p, bias, stream);
+  };
+  if (width == 16) go(pa_bwd_go<64, 16>, pa_bwd_go<128, 16>);
+  else if (width == 4) go(pa_bwd_go<64, 4>, pa_bwd_go<128, 4>);
+  else go(pa_bwd_go<64, 2>, pa_bwd_go<128, 2>);
   if (bias && dtable)
     hipLaunchKernelGGL(pa_table_grad_kernel, dim3(p->H), dim3(PA_BLOCK), 0,
-                       stream, p->part, dtable, dtable_bf16, items, p->H,
-                       bias->buckets);
+                       stream, p->part, dtable, dtable_bf16,
+                       (long)p->work_kv.n_chunks, p->H, bias->buckets);
 }

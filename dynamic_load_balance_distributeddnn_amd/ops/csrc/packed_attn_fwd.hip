@@ -7,32 +7,65 @@
 // [n, n] scores are never stored.  A workgroup owns 128 query rows of one
 // head, 32 a wave, and streams 64-key tiles through LDS; S is computed
 // transposed (keys x queries) so that a lane holds one query's scores and
-// the softmax needs one lane exchange a tile.  Rows of a sequence are
-// found through the packing's item list, longest first.
+// the softmax needs one lane exchange a tile.  The packing's list says
+// which rows and keys, most work first; a tile whose keys are shared out
+// to several workgroups is put together by a second kernel.
 #include "packed_attn.h"
 
-template <int DP, bool VEC, bool BIAS, typename BiasArg>
+// A row's end: its output and its statistics.
+template <int DP, int W, bool BIAS>
+__device__ PA_INLINE void pa_fwd_end(const PaFwd& p, long first, int row,
+                                     int len, int h, f32x16 (&acc)[DP / 32],
+                                     float m, float l) {
+  if (row >= len) return;
+  const int half = (threadIdx.x & 63) >> 5;
+  // no weight anywhere (a bias of -inf on all a row sees): zeros, and
+  // statistics under which the backward's weights are 0 too
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  __bf16* ob = static_cast<__bf16*>(p.o) + ((first + row) * p.H + h) * p.D;
+#pragma unroll
+  for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      bf16x4 v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = (__bf16)(acc[t][4 * g + e] * inv);
+      pa_store4<W>(ob, t * 32 + 8 * g + 4 * half, p.D, v);
+    }
+  if (half == 0) {
+    const long at = (long)h * p.T + first + row;
+    const float lg = l == 0.f ? INFINITY : __builtin_amdgcn_logf(l);
+    const float top = m == -INFINITY ? 0.f : m;
+    if constexpr (BIAS) {
+      p.stats[2 * at] = top;
+      p.stats[2 * at + 1] = lg;
+    } else {
+      p.stats[at] = top * (p.scale * PA_LOG2E) + lg;
+    }
+  }
+}
+
+template <int DP, int W, bool BIAS, typename BiasArg>
 __global__ void __launch_bounds__(PA_BLOCK, 2)
 pa_fwd_kernel(const PaFwd p, const BiasArg bias) {
   const int KS = DP / 16, DT = DP / 32;
-  __shared__ __attribute__((aligned(16))) __bf16 s_k[2][PA_STEP * DP];
-  __shared__ __attribute__((aligned(16))) __bf16 s_v[2][PA_STEP * DP];
+  const int TILE = PA_STEP * DP;
+  __shared__ __attribute__((aligned(1024))) __bf16 s_tiles[4][TILE];
+  __bf16 (*s_k)[TILE] = s_tiles, (*s_v)[TILE] = s_tiles + 2;
   __shared__ float s_win[BIAS ? 2 : 1][BIAS ? 192 : 1];
   __shared__ float s_tab[BIAS ? PA_MAXBUCKETS : 1];
   __shared__ int s_start[BIAS ? PA_MAXBUCKETS : 1];
 
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5;
   const int h = pa_head(blockIdx.x % p.H, p.H);
-  const PaItem it = p.items[blockIdx.x / p.H];
+  const PaChunk it = p.work.chunks[blockIdx.x / p.H];
   const int r0 = it.tile * PA_ROWS;
   const int w0 = r0 + wave * 32;     // this wave's first row
   const int row = w0 + col;          // this lane's
   const int len = it.len;
-  const int tiles = (min(r0 + PA_ROWS, len) + PA_STEP - 1) / PA_STEP;
-  const __bf16* kb = pa_at(p.k, it.first, h / p.G);
-  const __bf16* vb = pa_at(p.v, it.first, h / p.G);
-
+  const int whole = r0 / PA_STEP;  // tiles that all rows see whole
   float far_bias = 0.f;
   int far_from = 0;
   if constexpr (BIAS) {
@@ -45,7 +78,7 @@ pa_fwd_kernel(const PaFwd p, const BiasArg bias) {
     far_from = s_start[bias.buckets - 1];
   }
   // bias of the distances a 128 x 64 tile spans, r0 - k0 - 63 upwards
-  auto window = [&](int k0) {
+  auto window = [&](int k0) PA_INLINE {
     float x = 0.f;
     if constexpr (BIAS) {
       const int n = r0 - k0 - (PA_STEP - 1) + (int)threadIdx.x;
@@ -53,17 +86,16 @@ pa_fwd_kernel(const PaFwd p, const BiasArg bias) {
     }
     return x;
   };
-  auto near = [&](int k0) { return r0 - k0 - (PA_STEP - 1) < far_from; };
+  auto near = [&](int k0) PA_INLINE {
+    return r0 - k0 - (PA_STEP - 1) < far_from;
+  };
 
   bf16x8 qf[KS];
   {
     const __bf16* qb = pa_at(p.q, (long)it.first + min(row, len - 1), h);
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      const int d = s * 16 + half * 8;
-      qf[s] = pa_load8<VEC>(qb + (VEC ? min(d, p.D - 8) : min(d, p.D - 1)),
-                            p.D - d);
-    }
+    for (int s = 0; s < KS; ++s)
+      qf[s] = pa_load8<W>(qb, s * 16 + half * 8, p.D);
   }
 
   f32x16 acc[DT];
@@ -73,173 +105,237 @@ pa_fwd_kernel(const PaFwd p, const BiasArg bias) {
   float l = 0.f;         // this half's part of the sum
   const float to2 = BIAS ? PA_LOG2E : p.scale * PA_LOG2E;
 
-  PaStage<DP, VEC> ks, vs;
+  PaStage<DP, W> ks{pa_at(p.k, it.first, h / p.G), p.k.row, len, p.D};
+  PaStage<DP, W> vs{pa_at(p.v, it.first, h / p.G), p.v.row, len, p.D};
   float win = 0.f;
-  ks.load(kb, p.k.row, 0, len, p.D);
-  vs.load(vb, p.v.row, 0, len, p.D);
-  ks.store(s_k[0]);
-  vs.store(s_v[0]);
-  if constexpr (BIAS) {
-    if (threadIdx.x < 192) s_win[0][threadIdx.x] = window(0);
+  auto start = [&](int k0, int buf) PA_INLINE {
+    ks.start(k0, s_k[buf]);
+    vs.start(k0, s_v[buf]);
+    if (BIAS && near(k0)) win = window(k0);
+  };
+  auto arrive = [&](int k0, int buf) PA_INLINE {
+    if (BIAS && near(k0) && threadIdx.x < 192) s_win[buf][threadIdx.x] = win;
+    ks.arrive(k0, s_k[buf]);
+    vs.arrive(k0, s_v[buf]);
+    __syncthreads();
+  };
+  if (p.D < DP) {
+    pa_clear<DP>(s_k[0], 2 * PA_STEP);
+    pa_clear<DP>(s_v[0], 2 * PA_STEP);
+    __syncthreads();
   }
-  bool bad = __syncthreads_or(PA_STEP > r0 && vs.nonfinite());
+  start(it.begin * PA_STEP, it.begin & 1);
+  arrive(it.begin * PA_STEP, it.begin & 1);
 
-  for (int t = 0; t < tiles; ++t) {
-    const int k0 = t * PA_STEP, buf = t & 1;
-    const bool more = t + 1 < tiles;
-    if (more) {
-      ks.load(kb, p.k.row, k0 + PA_STEP, len, p.D);
-      vs.load(vb, p.v.row, k0 + PA_STEP, len, p.D);
-      if (BIAS && near(k0 + PA_STEP)) win = window(k0 + PA_STEP);
+  const PaFrags<DP> lanes(s_tiles, lane);
+  PaFrags<DP> frags = lanes;  // of the current buffer
+  auto scores = [&](f32x16 (&s)[2], int k0, int buf) PA_INLINE {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      s[j] = pa_zero16();
+#pragma unroll
+      for (int x = 0; x < KS; ++x)
+        s[j] = pa_mfma(frags.rows(j * 32 * DP * 2, x),
+                       qf[x], s[j]);
     }
-    if (bad) {
-      pa_poison<DP, true>(s_v[buf], acc, row - k0, lane);
-      __syncthreads();
-      pa_cleanse<DP>(s_v[buf]);
-      __syncthreads();
-    }
-    if (k0 <= w0 + 31) {
-      f32x16 s[2];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        s[j] = pa_zero16();
-#pragma unroll
-        for (int x = 0; x < KS; ++x)
-          s[j] = pa_mfma(pa_row_frag<DP>(s_k[buf], j * 32 + col,
-                                         2 * x + half), qf[x], s[j]);
-      }
-      if constexpr (BIAS) {
-        if (near(k0)) {
-          const float* w = s_win[buf] + wave * 32 + col + (PA_STEP - 1);
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-              s[j][r] = fmaf(s[j][r], p.scale,
-                             w[-(j * 32 + 8 * (r >> 2) + 4 * half + (r & 3))]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-              s[j][r] = fmaf(s[j][r], p.scale, far_bias);
-        }
-      }
-      if (k0 + PA_STEP - 1 > w0) {
-        const int lim = row - k0 - 4 * half;
+    if constexpr (BIAS) {
+      if (near(k0)) {
+        const float* w = s_win[buf] + wave * 32 + col + (PA_STEP - 1);
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int r = 0; r < 16; ++r)
-            if (j * 32 + 8 * (r >> 2) + (r & 3) > lim) s[j][r] = -INFINITY;
-      }
-      float top = -INFINITY;
+            s[j][r] = fmaf(s[j][r], p.scale,
+                           w[-(j * 32 + 8 * (r >> 2) + 4 * half + (r & 3))]);
+      } else {
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[j][r]);
-      top = fmaxf(m, pa_half_max(top));
-      // The sum and the output are held relative to m; they are scaled
-      // anew only when a maximum grew by more than 2^8, which fp32 and
-      // the bf16 weights (their step is relative) carry without loss.
-      if (__any((top - m) * to2 > 8.f || m == -INFINITY)) {
-        const float now = top == -INFINITY ? 0.f : top;
-        const float f = __builtin_amdgcn_exp2f((m - now) * to2);
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) acc[d][r] *= f;
-        l *= f;
-        m = top;
-      }
-      const float ref = m == -INFINITY ? 0.f : m;
-      const float off = ref * to2;
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          // with a bias the scores may stand at the type's lowest value:
-          // the difference is taken before the change of base
-          const float e = BIAS ? (s[j][r] - ref) * to2
-                               : fmaf(s[j][r], to2, -off);
-          s[j][r] = __builtin_amdgcn_exp2f(e);
-          l += s[j][r];
-        }
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const bf16x8 w = pa_operand(s[x >> 1], x & 1);
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-          acc[d] = pa_mfma(pa_col_frag<DP>(s_v[buf], x * 16, d * 32, lane), w,
-                           acc[d]);
+          for (int r = 0; r < 16; ++r)
+            s[j][r] = fmaf(s[j][r], p.scale, far_bias);
       }
     }
-    if (more) {
-      ks.store(s_k[buf ^ 1]);
-      vs.store(s_v[buf ^ 1]);
-      if (BIAS && near(k0 + PA_STEP) && threadIdx.x < 192)
-        s_win[buf ^ 1][threadIdx.x] = win;
-      if (k0 + 2 * PA_STEP > r0)
-        bad = __syncthreads_or(vs.nonfinite());
-      else
+  };
+  auto maximum = [&](const f32x16 (&s)[2]) PA_INLINE {
+    float top = s[0][0];
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[j][r]);
+    return fmaxf(m, pa_half_max(top));
+  };
+  auto weights = [&](f32x16 (&s)[2], float ref) PA_INLINE {
+    const float off = ref * to2;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        // with a bias the scores may stand at the type's lowest value: the
+        // difference is taken before the change of base
+        const float e = BIAS ? (s[j][r] - ref) * to2
+                             : fmaf(s[j][r], to2, -off);
+        s[j][r] = __builtin_amdgcn_exp2f(e);
+        l += s[j][r];
+      }
+  };
+  auto values = [&](const f32x16 (&s)[2]) PA_INLINE {
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const bf16x8 w = pa_operand(s[x >> 1], x & 1);
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+        acc[d] = pa_mfma(
+            frags.cols((2 * PA_STEP + x * 16) * DP * 2, d), w,
+            acc[d]);
+    }
+  };
+
+  // Any tile: with keys ahead of some row, and with a new maximum.
+  auto any_tile = [&](int t) PA_INLINE {
+    const int k0 = t * PA_STEP, buf = t & 1;
+    const bool more = t + 1 < it.end;
+    if (more) start(k0 + PA_STEP, buf ^ 1);
+    if (t >= whole) {
+      if (__syncthreads_or(pa_tile_nonfinite<DP, PA_STEP>(s_v[buf]))) {
+        pa_poison<DP, PA_STEP, true>(s_v[buf], acc, row - k0, lane);
         __syncthreads();
+        pa_cleanse<DP, PA_STEP>(s_v[buf]);
+        __syncthreads();
+      }
     }
+    frags = lanes.fresh(buf * TILE * 2);
+    if (k0 <= w0 + 31) {
+      f32x16 s[2];
+      scores(s, k0, buf);
+      const int lim = row - k0 - 4 * half;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (j * 32 + 8 * (r >> 2) + (r & 3) > lim) s[j][r] = -INFINITY;
+      const float top = maximum(s);
+      const float ref = top == -INFINITY ? 0.f : top;
+      const float f = __builtin_amdgcn_exp2f((m - ref) * to2);
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[d][r] *= f;
+      l *= f;
+      m = top;
+      weights(s, ref);
+      values(s);
+    }
+    if (more) arrive(k0 + PA_STEP, buf ^ 1);
+  };
+
+  // A tile that all rows see whole, with the maximum as it is held: the
+  // sum and the output are scaled anew only once a maximum grew by more
+  // than 2^16, which fp32 and the bf16 weights (their step is relative)
+  // carry without loss.  False, with nothing done, where it did; the
+  // wave then goes on with any_tile, which has as many barriers.
+  auto whole_tile = [&](int t) PA_INLINE {
+    const int k0 = t * PA_STEP, buf = t & 1;
+    const bool more = t + 1 < it.end;
+    if (more) start(k0 + PA_STEP, buf ^ 1);
+    frags = lanes.fresh(buf * TILE * 2);
+    f32x16 s[2];
+    scores(s, k0, buf);
+    if (__any((maximum(s) - m) * to2 > 16.f)) return false;
+    weights(s, m == -INFINITY ? 0.f : m);
+    values(s);
+    if (more) arrive(k0 + PA_STEP, buf ^ 1);
+    return true;
+  };
+
+  const int fast = min(whole, it.end);
+  for (int t = it.begin; t < it.end;) {
+    any_tile(t++);
+    if (t == it.begin + 1)
+      while (t < fast && whole_tile(t)) ++t;
   }
 
   l = pa_half_sum(l);
-  if (row >= len) return;
-  // no weight anywhere (a bias of -inf on all a row sees): zeros, and
-  // statistics under which the backward's weights are 0 too
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  __bf16* ob = static_cast<__bf16*>(p.o) +
-               (((long)it.first + row) * p.H + h) * p.D;
+  if (it.slot >= 0) {
 #pragma unroll
-  for (int t = 0; t < DT; ++t)
+    for (int t = 0; t < DT; ++t)
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int d = t * 32 + 8 * g + 4 * half;
-      bf16x4 v;
+      for (int g = 0; g < 4; ++g)
+        *pa_sums(p.work, it.slot, p.H, h, DT * 4, t * 4 + g) =
+            f32x4{acc[t][4 * g], acc[t][4 * g + 1], acc[t][4 * g + 2],
+                  acc[t][4 * g + 3]};
+    if (half == 0) {
+      float* to = pa_rows(p.work, it.slot, p.H, h, wave * 32 + col);
+      to[0] = m;
+      to[1] = l;
+    }
+    return;
+  }
+  pa_fwd_end<DP, W, BIAS>(p, it.first, row, len, h, acc, m, l);
+}
+
+// Tiles in several chunks: with the largest maximum of a row,
+// O = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i.
+template <int DP, int W, bool BIAS>
+__global__ void __launch_bounds__(PA_BLOCK)
+pa_fwd_join_kernel(const PaFwd p) {
+  const int DT = DP / 32;
+  const int h = blockIdx.x % p.H;
+  const PaJoin j = p.work.joins[blockIdx.x / p.H];
+  const int in = (threadIdx.x >> 6) * 32 + (threadIdx.x & 31);
+  const float to2 = BIAS ? PA_LOG2E : p.scale * PA_LOG2E;
+  float m = -INFINITY, l = 0.f;
+  for (int i = 0; i < j.n; ++i)
+    m = fmaxf(m, pa_rows(p.work, j.slot + i, p.H, h, in)[0]);
+  const float ref = m == -INFINITY ? 0.f : m;
+  f32x16 acc[DT];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = (__bf16)(acc[t][4 * g + e] * inv);
-      if (VEC) {
-        if (d < p.D) *reinterpret_cast<bf16x4*>(ob + d) = v;
-      } else {
+  for (int t = 0; t < DT; ++t) acc[t] = pa_zero16();
+  for (int i = 0; i < j.n; ++i) {
+    const float* from = pa_rows(p.work, j.slot + i, p.H, h, in);
+    const float f = __builtin_amdgcn_exp2f((from[0] - ref) * to2);
+    l += f * from[1];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (d + e < p.D) ob[d + e] = v[e];
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 x =
+            *pa_sums(p.work, j.slot + i, p.H, h, DT * 4, t * 4 + g);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[t][4 * g + e] += f * x[e];
       }
-    }
-  if (half == 0) {
-    const long at = (long)h * p.T + it.first + row;
-    const float lg = l == 0.f ? INFINITY : __builtin_amdgcn_logf(l);
-    if constexpr (BIAS) {
-      p.stats[2 * at] = m == -INFINITY ? 0.f : m;
-      p.stats[2 * at + 1] = lg;
-    } else {
-      p.stats[at] = (m == -INFINITY ? 0.f : m * to2) + lg;
-    }
+  }
+  pa_fwd_end<DP, W, BIAS>(p, j.first, j.tile * PA_ROWS + in, j.len, h, acc, m,
+                          l);
+}
+
+template <int DP, int W>
+static void pa_fwd_go(const PaFwd& p, const PaBias* bias,
+                      hipStream_t stream) {
+  const dim3 grid((unsigned)p.work.n_chunks * p.H), block(PA_BLOCK);
+  const dim3 joins((unsigned)p.work.n_joins * p.H);
+  if (bias) {
+    hipLaunchKernelGGL((pa_fwd_kernel<DP, W, true, PaBias>), grid, block, 0,
+                       stream, p, *bias);
+    if (joins.x)
+      hipLaunchKernelGGL((pa_fwd_join_kernel<DP, W, true>), joins, block, 0,
+                         stream, p);
+  } else {
+    hipLaunchKernelGGL((pa_fwd_kernel<DP, W, false, PaNoBias>), grid, block,
+                       0, stream, p, PaNoBias{});
+    if (joins.x)
+      hipLaunchKernelGGL((pa_fwd_join_kernel<DP, W, false>), joins, block, 0,
+                         stream, p);
   }
 }
 
-template <int DP, bool VEC>
-static void pa_fwd_go(const PaFwd& p, const PaBias* bias, unsigned grid,
-                      hipStream_t stream) {
-  if (bias)
-    hipLaunchKernelGGL((pa_fwd_kernel<DP, VEC, true, PaBias>), dim3(grid),
-                       dim3(PA_BLOCK), 0, stream, p, *bias);
-  else
-    hipLaunchKernelGGL((pa_fwd_kernel<DP, VEC, false, PaNoBias>), dim3(grid),
-                       dim3(PA_BLOCK), 0, stream, p, PaNoBias{});
-}
-
-// vec: head size, strides and addresses allow 16-byte loads.
+// width: 16, 4 or 2 bytes, what the head size, strides and addresses of
+// all tensors are multiples of.
 extern "C" void dlb_packed_attn_fwd(const PaFwd* p, const PaBias* bias,
-                                    long items, int vec, hipStream_t stream) {
-  const unsigned grid = (unsigned)(items * p->H);
-  if (p->D <= 64)
-    vec ? pa_fwd_go<64, true>(*p, bias, grid, stream)
-        : pa_fwd_go<64, false>(*p, bias, grid, stream);
-  else
-    vec ? pa_fwd_go<128, true>(*p, bias, grid, stream)
-        : pa_fwd_go<128, false>(*p, bias, grid, stream);
+                                    int width, hipStream_t stream) {
+  auto go = [&](auto go64, auto go128) {
+    (p->D <= 64 ? go64 : go128)(*p, bias, stream);
+  };
+  if (width == 16) go(pa_fwd_go<64, 16>, pa_fwd_go<128, 16>);
+  else if (width == 4) go(pa_fwd_go<64, 4>, pa_fwd_go<128, 4>);
+  else go(pa_fwd_go<64, 2>, pa_fwd_go<128, 2>);
 }

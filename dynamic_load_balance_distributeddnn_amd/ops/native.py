@@ -297,11 +297,11 @@ class _PackedCausalAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, table, packing, scale, starts):
-        items, _ = packing.tables(q.device)
+        work, _ = packing.work(q.device, q.shape[1], k.shape[1])
         q, k, v = (t if t.shape[-1] == 1 or t.stride(-1) == 1
                    else t.contiguous() for t in (q, k, v))
         flat = None if table is None else table.detach().contiguous()
-        o, stats = ext().packed_attn_fwd(q, k, v, items, packing.total,
+        o, stats = ext().packed_attn_fwd(q, k, v, work, packing.total,
                                          scale, flat, starts)
         ctx.save_for_backward(q, k, v, o, stats, flat)
         ctx.attn_args = (packing, scale, starts)
@@ -312,12 +312,12 @@ class _PackedCausalAttention(torch.autograd.Function):
     def backward(ctx, do):
         q, k, v, o, stats, flat = ctx.saved_tensors
         packing, scale, starts = ctx.attn_args
-        items, items_kv = packing.tables(q.device)
+        work_q, work_kv = packing.work(q.device, q.shape[1], k.shape[1])
         if do.shape[-1] != 1 and do.stride(-1) != 1:
             do = do.contiguous()
-        grads = ext().packed_attn_bwd(q, k, v, o, stats, do, items, items_kv,
-                                      packing.total, scale, flat, starts,
-                                      ctx.needs_input_grad[3])
+        grads = ext().packed_attn_bwd(q, k, v, o, stats, do, work_q,
+                                      work_kv, packing.total, scale, flat,
+                                      starts, ctx.needs_input_grad[3])
         dtable = grads[3] if ctx.needs_input_grad[3] else None
         return grads[0], grads[1], grads[2], dtable, None, None, None
 

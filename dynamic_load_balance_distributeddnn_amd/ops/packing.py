@@ -26,10 +26,8 @@ class PackedSequences:
     and use it for all layers, forward and backward, on any stream; it has
     to outlive a captured graph that used it.
 
-    On the device it keeps two work lists of 128-row tiles, the ones with
-    most to do first: for the queries (a tile reads the keys up to its
-    last row) and for the keys (a tile is read by the rows from its first
-    on).
+    For each head layout it is used with it keeps two work lists on the
+    device, of the query tiles and of the key tiles (``work``).
     """
 
     def __init__(self, lengths, device=None):
@@ -52,47 +50,91 @@ class PackedSequences:
         self.lengths = tuple(n.tolist())
         self.offsets = (0, *np.cumsum(n).tolist())
         self.total = self.offsets[-1]
-        self._tables = {}
-        if device is not None and torch.device(device).type == "cuda":
-            self.tables(device)
+        self.device = None if device is None else torch.device(device)
+        self._lists = {}
 
     def __len__(self):
         return len(self.lengths)
 
-    def _host_tables(self):
-        n = self._n
-        tiles = -(-n // TILE_ROWS)
-        seq = np.repeat(np.arange(len(n)), tiles)
-        first_tile = np.cumsum(tiles) - tiles
-        tile = np.arange(len(seq)) - first_tile[seq]
-        items = np.zeros((len(seq), 4), np.int32)
-        items[:, 0] = np.asarray(self.offsets[:-1], np.int64)[seq]
-        items[:, 1] = n[seq]
-        items[:, 2] = tile
-        seen = np.minimum((tile + 1) * TILE_ROWS, n[seq])
-        seeing = n[seq] - tile * TILE_ROWS
-        return np.stack([items[np.argsort(-seen, kind="stable")],
-                         items[np.argsort(-seeing, kind="stable")]])
+    def _tiles(self):
+        """(sequence, tile) of every 128-row tile."""
+        tiles = -(-self._n // TILE_ROWS)
+        seq = np.repeat(np.arange(len(tiles)), tiles)
+        return seq, np.arange(len(seq)) - (np.cumsum(tiles) - tiles)[seq]
 
-    def tables(self, device):
-        """(query tiles, key tiles), int32 [tiles, 4] each: the sequence's
-        first row, its length, the tile, unused."""
-        device = torch.device(device)
-        if device.index is None:
-            device = torch.device(device.type, torch.cuda.current_device())
-        if device not in self._tables:
+    def host_work(self, heads, kv_heads):
+        """((list, chunks, slots) of the query tiles, of the key tiles).
+
+        A query tile reads the 64-key tiles up to its last row; a key tile
+        is read by the 32-row tiles from its first row on, of every head
+        that shares it.  Tiles with much more to do than a workgroup's
+        share of the whole are cut into chunks, whose sums a second kernel
+        joins; the chunks come with the longest first.
+        """
+        seq, tile = self._tiles()
+        n = self._n[seq]
+        keys = -(-np.minimum((tile + 1) * TILE_ROWS, n) // 64)
+        queries = -(-(n - tile * TILE_ROWS) // 32) * (heads // kv_heads)
+        return (self._chunks(seq, tile, keys, heads, 8, 512),
+                self._chunks(seq, tile, queries, kv_heads, 16, 768))
+
+    def _chunks(self, seq, tile, steps, heads, least, shares):
+        # 512 workgroups run at a time, so the longest tile is what a launch
+        # takes at least.  Cutting costs a trip of the sums through memory:
+        # one sequence of 4001, 12 heads of 64, forward 85 -> 63 us where
+        # the longest is 2.7 times a place's share, but 7 packed ones,
+        # 16 heads of 128, 90 -> 100 us where it is 1.3 times.  The key
+        # tiles, longer and more uneven, want shorter chunks: one of 8192,
+        # 32 heads of 128 over 8, backward uncut 2740 us, 512 shares 2260,
+        # 768 shares 2120, 1024 shares 2190.
+        total = int(steps.sum()) * heads
+        limit = max(least, total // shares)
+        if len(steps) and int(steps.max()) <= 1.5 * total / 512:
+            limit = int(steps.max())
+        parts = -(-steps // limit)
+        which = np.repeat(np.arange(len(steps)), parts)
+        part = np.arange(len(which)) - (np.cumsum(parts) - parts)[which]
+        cut = parts > 1
+        slots = np.cumsum(parts * cut) - parts * cut
+        rows = np.zeros((len(which) + int(cut.sum()), 8), np.int32)
+        first = np.asarray(self.offsets[:-1], np.int64)[seq]
+        chunks, joins = rows[:len(which)], rows[len(which):]
+        chunks[:, 0] = first[which]
+        chunks[:, 1] = self._n[seq[which]]
+        chunks[:, 2] = tile[which]
+        chunks[:, 3] = part * steps[which] // parts[which]
+        chunks[:, 4] = (part + 1) * steps[which] // parts[which]
+        chunks[:, 5] = np.where(cut[which], slots[which] + part, -1)
+        chunks[:] = chunks[np.argsort(chunks[:, 3] - chunks[:, 4],
+                                      kind="stable")]
+        joins[:, 0] = first[cut]
+        joins[:, 1] = self._n[seq[cut]]
+        joins[:, 2] = tile[cut]
+        joins[:, 3] = slots[cut]
+        joins[:, 4] = parts[cut]
+        return rows, len(which), int((parts * cut).sum())
+
+    def work(self, device, heads, kv_heads):
+        """The work lists of one head layout on a device, made at its first
+        use (not within a graph capture) and kept."""
+        key = (device, heads, kv_heads)
+        if key not in self._lists:
             if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("build the PackedSequences for its device "
-                                   "before the capture")
-            # a synchronous copy: the tables are there for every stream
-            both = torch.from_numpy(self._host_tables()).to(device)
-            self._tables[device] = (
+                raise RuntimeError("use the PackedSequences once with these "
+                                   "heads before the capture")
+            lists = self.host_work(heads, kv_heads)
+            both = np.concatenate([rows for rows, _, _ in lists])
+            # a synchronous copy: the lists are there for every stream
+            both = torch.from_numpy(both).to(device)
+            cut = len(lists[0][0])
+            self._lists[key] = (
+                (both[:cut], *lists[0][1:]), (both[cut:], *lists[1][1:]),
                 both, torch.cuda.current_stream(device))
-        both, made_on = self._tables[device]
+        queries, keys, both, made_on = self._lists[key]
         now = torch.cuda.current_stream(device)
         if now != made_on:
             both.record_stream(now)
-        return both[0], both[1]
+        return queries, keys
 
 
 @lru_cache(maxsize=64)

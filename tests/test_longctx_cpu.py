@@ -99,25 +99,47 @@ def test_plain_bias(both):
         lambda t: FD.relative_position_bias(t, 6, 20, 12, both), table)
 
 
-def test_work_lists():
-    """Every row of every sequence in one tile, most work first."""
-    lens = [5, 0, TILE_ROWS, TILE_ROWS + 1, 1000]
-    pack = FD.PackedSequences(torch.tensor(lens))
-    assert pack.total == sum(lens) and len(pack) == 5
-    queries, keys = pack._host_tables()
-    for items in (queries, keys):
-        rows = set()
-        for first, n, tile, _ in items.tolist():
-            assert (first, n) in zip(pack.offsets, lens)
-            top = min(n, (tile + 1) * TILE_ROWS)
-            assert tile * TILE_ROWS < n
-            rows |= {first + r for r in range(tile * TILE_ROWS, top)}
-        assert rows == set(range(sum(lens)))
-        assert len(items) == sum(-(-n // TILE_ROWS) for n in lens)
-    seen = [min(n, (t + 1) * TILE_ROWS) for _, n, t, _ in queries.tolist()]
-    seeing = [n - t * TILE_ROWS for _, n, t, _ in keys.tolist()]
-    assert seen == sorted(seen, reverse=True)
-    assert seeing == sorted(seeing, reverse=True)
+@pytest.mark.parametrize("heads,kv", [(1, 1), (32, 8), (16, 16)])
+@pytest.mark.parametrize("lens", [
+    [5, 0, TILE_ROWS, TILE_ROWS + 1, 1000], [1], [], [9000],
+    [3000, 1, 2500, 300, 77]])
+def test_work_lists(lens, heads, kv):
+    """Every step of every tile is in one chunk, the longest chunks come
+    first, and the chunks of a cut tile have places of their own next to
+    each other, which its join names."""
+    pack = FD.PackedSequences(torch.tensor(lens, dtype=torch.long))
+    assert pack.total == sum(lens) and len(pack) == len(lens)
+    for keys, (rows, n, slots) in enumerate(pack.host_work(heads, kv)):
+        chunks, joins = rows[:n].tolist(), rows[n:].tolist()
+        size = [c[4] - c[3] for c in chunks]
+        assert size == sorted(size, reverse=True)
+        steps, places = {}, {}
+        for first, length, tile, begin, end, slot, _, _ in chunks:
+            assert (first, length) in zip(pack.offsets, lens)
+            assert begin < end
+            steps.setdefault((first, tile), []).append((begin, end))
+            places.setdefault((first, tile), []).append((begin, slot))
+        for (first, length) in zip(pack.offsets, lens):
+            for tile in range(-(-length // TILE_ROWS)):
+                if keys:
+                    want = -(-(length - tile * TILE_ROWS) // 32)
+                    want *= heads // kv
+                else:
+                    want = -(-min((tile + 1) * TILE_ROWS, length) // 64)
+                at = 0
+                for begin, end in sorted(steps.pop((first, tile))):
+                    assert begin == at
+                    at = end
+                assert at == want
+                assert keys or tile or len(places[first, tile]) == 1
+        assert not steps
+        used = []
+        for first, length, tile, slot, count, _, _, _ in joins:
+            at = [s for _, s in sorted(places.pop((first, tile)))]
+            assert at == list(range(slot, slot + count)) and count > 1
+            used += at
+        assert sorted(used) == list(range(slots))
+        assert all(s == [(0, -1)] for s in places.values())
 
 
 @pytest.mark.parametrize("lengths,error", [
