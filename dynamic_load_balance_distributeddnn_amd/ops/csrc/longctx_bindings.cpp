@@ -1,6 +1,8 @@
 // Python bindings of packed causal attention and of the position bias.
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
 #include "longctx_args.h"
@@ -270,7 +272,112 @@ static Tensor relbias_bwd(Tensor dout, Tensor table,
   return dtable;
 }
 
+// ---- autograd.  In C++, where a call and its gradient cost the host a
+// third of what Python functions do: small sequences are bound by it.
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// Gradients under create_graph: differentiating them again is an error.
+static variable_list once(variable_list grads, const char* name) {
+  if (!at::GradMode::is_enabled()) return grads;
+  auto error = std::make_shared<torch::autograd::DelayedError>(
+      std::string(name) + " can be differentiated once only",
+      (int64_t)grads.size());
+  for (auto& g : grads)
+    if (g.defined()) g = g.detach().requires_grad_();
+  return (*error)(std::move(grads));
+}
+
+static Tensor dense_last(const Tensor& t) {
+  return t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous();
+}
+
+struct PackedAttention
+    : public torch::autograd::Function<PackedAttention> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& q0,
+                        const Tensor& k0, const Tensor& v0,
+                        const MaybeTensor& table0, WorkList work_q,
+                        WorkList work_kv, int64_t total, double scale,
+                        std::vector<int64_t> starts, bool table_grad) {
+    const Tensor q = dense_last(q0), k = dense_last(k0), v = dense_last(v0);
+    MaybeTensor table;
+    if (table0.has_value()) table = table0->contiguous();
+    auto out = packed_attn_fwd(q, k, v, work_q, total, scale, table, starts);
+    ctx->save_for_backward({q, k, v, out[0], out[1],
+                            table.has_value() ? *table : Tensor(),
+                            std::get<0>(work_q), std::get<0>(work_kv)});
+    auto& d = ctx->saved_data;
+    d["counts"] = std::vector<int64_t>{
+        std::get<1>(work_q), std::get<2>(work_q), std::get<1>(work_kv),
+        std::get<2>(work_kv), total};
+    d["scale"] = scale;
+    d["starts"] = std::move(starts);
+    d["table_grad"] = table_grad;
+    return out[0];
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grad) {
+    const auto saved = ctx->get_saved_variables();
+    auto& d = ctx->saved_data;
+    const auto n = d["counts"].toIntVector();
+    const bool table_grad = d["table_grad"].toBool();
+    MaybeTensor table;
+    if (saved[5].defined()) table = saved[5];
+    variable_list out(10);
+    {
+      at::AutoGradMode off(false);
+      auto grads = packed_attn_bwd(
+          saved[0], saved[1], saved[2], saved[3], saved[4],
+          dense_last(grad[0]), WorkList{saved[6], n[0], n[1]},
+          WorkList{saved[7], n[2], n[3]}, n[4], d["scale"].toDouble(), table,
+          d["starts"].toIntVector(), table_grad);
+      for (size_t i = 0; i < grads.size(); ++i) out[i] = grads[i];
+    }
+    return once(std::move(out), "packed_causal_attention");
+  }
+};
+
+static Tensor packed_attention(Tensor q, Tensor k, Tensor v,
+                               MaybeTensor table, WorkList work_q,
+                               WorkList work_kv, int64_t total, double scale,
+                               std::vector<int64_t> starts) {
+  return PackedAttention::apply(
+      q, k, v, table, work_q, work_kv, total, scale, starts,
+      table.has_value() && table->requires_grad());
+}
+
+struct PositionBias : public torch::autograd::Function<PositionBias> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& table, int64_t Q,
+                        int64_t K, std::vector<int64_t> starts,
+                        at::ScalarType type) {
+    ctx->save_for_backward({table});
+    auto out = relbias_fwd(table.to(type).contiguous(), Q, K, starts);
+    ctx->saved_data["starts"] = std::move(starts);
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grad) {
+    variable_list out(5);
+    {
+      at::AutoGradMode off(false);
+      out[0] = relbias_bwd(grad[0].contiguous(),
+                           ctx->get_saved_variables()[0],
+                           ctx->saved_data["starts"].toIntVector());
+    }
+    return once(std::move(out), "relative_position_bias");
+  }
+};
+
+static Tensor position_bias(Tensor table, int64_t Q, int64_t K,
+                            std::vector<int64_t> starts,
+                            py::object type) {
+  return PositionBias::apply(table, Q, K, starts,
+                             torch::python::detail::py_object_to_dtype(type));
+}
+
 void bind_longctx(py::module_& m) {
+  m.def("packed_attention", &packed_attention,
+        "causal attention over packed sequences, differentiable");
+  m.def("position_bias", &position_bias,
+        "bucketed position bias as a grid, differentiable in its table");
   m.def("packed_attn_fwd", &packed_attn_fwd,
         "causal attention over packed sequences");
   m.def("packed_attn_bwd", &packed_attn_bwd,

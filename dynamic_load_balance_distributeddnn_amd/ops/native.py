@@ -8,7 +8,6 @@ view on a channels_last tensor.
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import ext
 
@@ -266,65 +265,19 @@ def causal_attention(q, k, v, nhead, dropout_p=0.0):
     return _CausalAttention.apply(q, k, v, nhead, dropout_p)
 
 
-# ------------------------------------------------- relative position bias
-class _RelativePositionBias(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, table, q_len, k_len, starts, dtype):
-        ctx.save_for_backward(table)
-        ctx.starts = starts
-        return ext().relbias_fwd(table.detach().to(dtype).contiguous(),
-                                 q_len, k_len, starts)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dout):
-        (table,) = ctx.saved_tensors
-        dtable = ext().relbias_bwd(dout.contiguous(), table, ctx.starts)
-        return dtable, None, None, None, None
-
-
+# ------------------------------- relative position bias, packed attention
+# Their autograd functions are in csrc/longctx_bindings.cpp.
 def relative_position_bias(table, q_len, k_len, starts):
     dtype = table.dtype
     if dtype == torch.float32 and torch.is_autocast_enabled("cuda"):
         dtype = torch.get_autocast_dtype("cuda")
-    return _RelativePositionBias.apply(table, q_len, k_len, starts, dtype)
-
-
-# ------------------------------------------------ packed causal attention
-class _PackedCausalAttention(torch.autograd.Function):
-    """Saves q, k, v, the output and one statistic a row (two with a
-    bias); the backward recomputes the weights from them."""
-
-    @staticmethod
-    def forward(ctx, q, k, v, table, packing, scale, starts):
-        work, _ = packing.work(q.device, q.shape[1], k.shape[1])
-        q, k, v = (t if t.shape[-1] == 1 or t.stride(-1) == 1
-                   else t.contiguous() for t in (q, k, v))
-        flat = None if table is None else table.detach().contiguous()
-        o, stats = ext().packed_attn_fwd(q, k, v, work, packing.total,
-                                         scale, flat, starts)
-        ctx.save_for_backward(q, k, v, o, stats, flat)
-        ctx.attn_args = (packing, scale, starts)
-        return o
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, do):
-        q, k, v, o, stats, flat = ctx.saved_tensors
-        packing, scale, starts = ctx.attn_args
-        work_q, work_kv = packing.work(q.device, q.shape[1], k.shape[1])
-        if do.shape[-1] != 1 and do.stride(-1) != 1:
-            do = do.contiguous()
-        grads = ext().packed_attn_bwd(q, k, v, o, stats, do, work_q,
-                                      work_kv, packing.total, scale, flat,
-                                      starts, ctx.needs_input_grad[3])
-        dtable = grads[3] if ctx.needs_input_grad[3] else None
-        return grads[0], grads[1], grads[2], dtable, None, None, None
+    return ext().position_bias(table, q_len, k_len, starts, dtype)
 
 
 def packed_causal_attention(q, k, v, packing, scale, table, starts):
-    return _PackedCausalAttention.apply(q, k, v, table, packing, scale,
-                                        starts)
+    work_q, work_kv = packing.work(q.device, q.shape[1], k.shape[1])
+    return ext().packed_attention(q, k, v, table, work_q, work_kv,
+                                  packing.total, scale, starts)
 
 
 # ------------------------------------------------------------ log_softmax

@@ -365,6 +365,24 @@ def test_only_what_is_asked_for():
     assert not o.requires_grad and torch.equal(o, want["o"])
 
 
+def test_second_derivatives_are_refused():
+    FD = _fd()
+    q, k, v, do, table = _inputs(40, 2, 2, 64, buckets=8)
+    packing = FD.PackedSequences([40], device="cuda")
+    want = _run(q, k, v, do, [40], table, far=16)
+    leaves = [t.requires_grad_() for t in (q, k, v, table)]
+    o = FD.packed_causal_attention(*leaves[:3], packing, bias_table=table,
+                                   max_distance=16)
+    grads = torch.autograd.grad(o, leaves, do, create_graph=True)
+    assert torch.equal(grads[0], want["dq"])
+    with pytest.raises(RuntimeError, match="once only"):
+        grads[0].float().sum().backward()
+    grid = FD.relative_position_bias(table, 9, 9, 16)
+    dtable, = torch.autograd.grad(grid.sum(), table, create_graph=True)
+    with pytest.raises(RuntimeError, match="once only"):
+        dtable.sum().backward()
+
+
 def test_refusals_on_the_gpu():
     FD = _fd()
     q, k, v, _, table = _inputs(10, 2, 2, 64, buckets=8)
