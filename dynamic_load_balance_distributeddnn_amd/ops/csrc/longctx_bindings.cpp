@@ -14,7 +14,7 @@ extern "C" void dlb_packed_attn_bwd(const PaBwd* p, const PaBias* bias,
                                     hipStream_t stream);
 extern "C" void dlb_relbias_fwd(const void* table, void* out, const RbArgs* a,
                                 int size, hipStream_t stream);
-extern "C" long dlb_relbias_bwd_blocks(const RbArgs* a);
+extern "C" long dlb_relbias_bwd_blocks(const RbArgs* a, int size);
 extern "C" void dlb_relbias_bwd(const void* dout, int type, float* part,
                                 void* dtable, int table_type, const RbArgs* a,
                                 hipStream_t stream);
@@ -260,12 +260,18 @@ static Tensor relbias_bwd(Tensor dout, Tensor table,
               dout.device() == table.device() && table.dim() == 2 &&
               table.size(1) == dout.size(0));
   c10::DeviceGuard guard(dout.device());
+  // the kernel wants 16 bytes in a row: keys in front of the first, whose
+  // gradient is 0, move no distance
+  if (dout.size(2) > 0 && dout.size(2) < 8)
+    dout = torch::constant_pad_nd(dout, {8 - dout.size(2), 0});
   const RbArgs a = rb_args(dout.size(0), dout.size(1), dout.size(2),
                            table.size(0), starts);
   auto dtable = torch::empty({table.size(0), a.H}, table.options());
   if (dout.numel() == 0) return dtable.zero_();
-  auto part = torch::empty({dlb_relbias_bwd_blocks(&a), a.H, table.size(0)},
-                           dout.options().dtype(torch::kFloat32));
+  auto part = torch::empty(
+      {dlb_relbias_bwd_blocks(&a, (int)dout.element_size()), a.H,
+       table.size(0)},
+      dout.options().dtype(torch::kFloat32));
   dlb_relbias_bwd(dout.data_ptr(), rb_type(dout), part.data_ptr<float>(),
                   dtable.data_ptr(), rb_type(table), &a, current_stream());
   launched();
