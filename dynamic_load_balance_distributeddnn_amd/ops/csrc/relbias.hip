@@ -21,19 +21,33 @@
 typedef __attribute__((ext_vector_type(4))) unsigned rb_vec;
 typedef rb_vec __attribute__((aligned(4))) rb_words;  // on any word
 
-__device__ inline int rb_bucket(const RbArgs& a, const int* starts, long n) {
-  int extra = 0;
-  if (n < 0) {
-    if (!a.both) return 0;
-    n = -n;
-    extra = a.side;
-  }
-  int lo = 0, hi = a.side;  // starts[lo] <= n < starts[hi]
-  while (hi - lo > 1) {
+__device__ inline int rb_bucket(const RbArgs& a, const int* starts, long far) {
+  const int n0 = (int)min(max(far, -(1l << 30)), 1l << 30);
+  if (n0 < 0 && !a.both) return 0;
+  const int n = abs(n0), extra = n0 < 0 ? a.side : 0;
+  // the first half of the buckets hold one distance each
+  int lo = a.side / 2, hi = a.side - 1;
+  if (n < lo) return n + extra;
+  if (n >= starts[hi]) return hi + extra;
+  while (hi - lo > 1) {  // starts[lo] <= n < starts[hi]
     const int mid = (lo + hi) >> 1;
     if (starts[mid] <= n) lo = mid; else hi = mid;
   }
   return lo + extra;
+}
+
+// Sum over a wave, in every lane.
+__device__ inline float rb_wave_sum(float v) {
+#define RB_STEP(CTRL, ROWS)                                              \
+  v += __builtin_bit_cast(                                               \
+      float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v),  \
+                                         CTRL, ROWS, 0xf, false));
+  RB_STEP(0x111, 0xf) RB_STEP(0x112, 0xf)  // row_shr:1, 2, 4, 8
+  RB_STEP(0x114, 0xf) RB_STEP(0x118, 0xf)
+  RB_STEP(0x142, 0xa) RB_STEP(0x143, 0xc)  // row_bcast:15, 31
+#undef RB_STEP
+  return __builtin_bit_cast(
+      float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
 // A workgroup writes `rows` rows of one head, 2^lanes vectors of each and
@@ -56,6 +70,7 @@ rb_fwd_kernel(const W* __restrict__ table, W* __restrict__ out,
   typedef __attribute__((ext_vector_type(N))) W Vec;
   __shared__ Vec s_vec[N * LIST];
   __shared__ int s_start[RB_MAXBUCKETS];
+  __shared__ W s_tab[RB_MAXBUCKETS];
   const int t = threadIdx.x;
   const long h = blockIdx.z;
   const long i0 = (long)blockIdx.y * rows;
@@ -64,16 +79,18 @@ rb_fwd_kernel(const W* __restrict__ table, W* __restrict__ out,
   // columns of all rows' vectors: jlo .. jlo + width + N - 2
   const long jlo = (long)blockIdx.x * width - (N - 1);
   for (int b = t; b < a.side; b += RB_BLOCK) s_start[b] = a.starts[b];
+  for (int b = t; b < a.buckets; b += RB_BLOCK)
+    s_tab[b] = table[(long)b * a.H + h];
   __syncthreads();
   // diagonal x: j - i = jlo - (i0 + nrows - 1) + x
   const long top = i0 + nrows - 1 + a.K - a.Q - jlo;  // distance at x = 0
   const int span = width + N + nrows;
   const int b0 = rb_bucket(a, s_start, top);
   const bool plain = b0 == rb_bucket(a, s_start, top - (span - 1));
-  Vec same = table[(long)b0 * a.H + h];
+  Vec same = s_tab[b0];
   if (!plain) {
     for (int x = t; x < span; x += RB_BLOCK)
-      s_diag[x] = table[(long)rb_bucket(a, s_start, top - x) * a.H + h];
+      s_diag[x] = s_tab[rb_bucket(a, s_start, top - x)];
     __syncthreads();
     for (int x = t; x + N <= span; x += RB_BLOCK) {
       Vec v;
@@ -242,37 +259,43 @@ rb_bwd_kernel(const T* __restrict__ dout, float* __restrict__ part,
   for (int e = 0; e < N; ++e) s_diag[wave][lane * N + e] = sum[e];
   __syncthreads();
 
-  // The diagonals of a bucket are neighbours: distance top - x.  Only the
-  // buckets that the wave's diagonals meet are looked at, one for most.
-  const long top = a.K - a.Q - d0, least = top - (SPAN - 1);
-  auto add = [&](int b, long xlo, long xhi) {  // diagonals xlo .. xhi - 1
-    const int first = (int)max(xlo, 0l);
-    const int stop = (int)min(xhi, (long)SPAN);
-    float v = 0.f;
-    for (int x = first + lane; x < stop; x += 64) v += s_diag[wave][x];
-    v = wave_reduce_sum(v);
-    if (lane == 0) s_sum[wave][b] = v;
-  };
-  if (from < last) {
-    if (top >= 0 || !a.both) {
-      // without `both`, keys ahead of the query count as distance 0
-      const int b1 = rb_bucket(a, s_start, max(top, 0l));
-      for (int b = rb_bucket(a, s_start, max(least, 0l)); b <= b1; ++b) {
-        const long lo = b == 0 && !a.both ? min(least, 0l) : s_start[b];
-        const long hi = b + 1 < a.side ? s_start[b + 1] : top + 1;
-        add(b, top - hi + 1, top - lo + 1);
+  // The diagonals of a bucket are neighbours: distance top - x.  A lane
+  // takes a bucket; what is long for one lane (the far bucket of most
+  // waves) the wave adds up together.
+  const long top = a.K - a.Q - d0;
+  if (from < last)
+    for (int b0 = 0; b0 < a.buckets; b0 += 64) {
+      const int b = b0 + lane;
+      int first = 0, stop = 0;  // diagonals first .. stop - 1
+      if (b < a.buckets) {
+        const bool back = b >= a.side;  // keys ahead of the query
+        const int s = back ? b - a.side : b;
+        const long none = (long)1 << 60;
+        // distances lo .. hi - 1; distance 0 is not ahead, and without
+        // `both` what is ahead counts as distance 0
+        const long lo = back ? max(s_start[s], 1)
+                             : s == 0 && !a.both ? -none : s_start[s];
+        const long hi = s + 1 < a.side ? s_start[s + 1] : none;
+        const long xlo = back ? top + lo : top - hi + 1;
+        const long xhi = back ? top + hi : top - lo + 1;
+        first = (int)min(max(xlo, 0l), (long)SPAN);
+        stop = (int)min(max(xhi, 0l), (long)SPAN);
       }
-    }
-    if (least < 0 && a.both) {
-      const int b1 = rb_bucket(a, s_start, least);
-      for (int b = rb_bucket(a, s_start, min(top, -1l)); b <= b1; ++b) {
-        const int s = b - a.side;
-        const long lo = max(s_start[s], 1);  // distance 0 is not ahead
-        const long hi = s + 1 < a.side ? s_start[s + 1] : 1 - least;
-        add(b, top + lo, top + hi);
+      const bool together = stop - first > 32;
+      float v = 0.f;
+      if (!together)
+        for (int x = first; x < stop; ++x) v += s_diag[wave][x];
+      for (unsigned long long m = __ballot(together); m; m &= m - 1) {
+        const int l = __builtin_ctzll(m);
+        const int x0 = __builtin_amdgcn_readlane(first, l);
+        const int x1 = __builtin_amdgcn_readlane(stop, l);
+        float w = 0.f;
+        for (int x = x0 + lane; x < x1; x += 64) w += s_diag[wave][x];
+        w = rb_wave_sum(w);
+        if (lane == l) v = w;
       }
+      if (b < a.buckets) s_sum[wave][b] = v;
     }
-  }
   __syncthreads();
   float* mine = part + ((long)blockIdx.x * a.H + h) * a.buckets;
   for (int b = threadIdx.x; b < a.buckets; b += RB_BLOCK)
@@ -299,9 +322,10 @@ rb_reduce_kernel(const float* __restrict__ part, T* __restrict__ dtable,
 
 static long rb_div(long a, long b) { return (a + b - 1) / b; }
 
-// Rows of a workgroup: as many as leave 1024 workgroups, within bounds.
+// Rows of a workgroup: as many as leave 512 workgroups, within bounds.
+// What a workgroup lays out costs as much as some 30 rows.
 static int rb_rows(const RbArgs& a, long strips, int least, int most) {
-  const long rows = a.H * strips * a.Q / 1024;
+  const long rows = a.H * strips * a.Q / 512;
   return (int)(rows < least ? least : rows > most ? most : rows);
 }
 
