@@ -1,6 +1,7 @@
 // Python bindings of packed causal attention and of the position bias.
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPCachingAllocator.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
@@ -90,6 +91,10 @@ static PaWork pa_work(const Tensor& list, int64_t chunks, int64_t slots,
                   chunks <= list.size(0) && slots >= 0 &&
                   list.size(0) * heads < (1l << 31),
               "packed attention: work list does not fit");
+  // the list was made on another stream, maybe: it is not to be used again
+  // before this one is done with it
+  c10::hip::HIPCachingAllocator::recordStream(list.storage().data_ptr(),
+                                              at::hip::getCurrentHIPStream());
   PaWork w{};
   w.chunks = static_cast<const PaChunk*>(list.data_ptr());
   w.joins = reinterpret_cast<const PaJoin*>(w.chunks + chunks);

@@ -258,6 +258,47 @@ def packed_causal_attention(q, k, v, packing, scale=None, bias_table=None,
     softmax statistics and the gradients' sums are fp32, and results do
     not change from run to run.  The table may be fp32 or bfloat16.
     """
+    if (q.dtype == torch.float32 and q.is_cuda
+            and torch.is_autocast_enabled("cuda")):
+        q, k, v = (t.to(torch.bfloat16) for t in (q, k, v))
+    qs, ks, dtype, device = q.shape, k.shape, q.dtype, q.device
+    if not (isinstance(packing, PackedSequences) and len(qs) == 3
+            and len(ks) == 3 and ks == v.shape and ks[0] == qs[0]
+            and ks[2] == qs[2] > 0 and ks[1] > 0 and qs[1] > 0
+            and qs[1] % ks[1] == 0 and packing.total <= qs[0]
+            and dtype.is_floating_point and k.dtype == dtype == v.dtype
+            and k.device == device == v.device):
+        _refuse_packed_attention(q, k, v, packing)
+    scale = qs[2] ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < math.inf:
+        raise ValueError(f"scale has to be positive and finite, got {scale}")
+    starts = ()
+    if bias_table is not None:
+        if bias_table.dim() != 2 or bias_table.shape[1] != qs[1]:
+            raise ValueError(
+                f"the bias table is [num_buckets, {qs[1]}], got "
+                f"{tuple(bias_table.shape)}")
+        if bias_table.device != device:
+            raise ValueError("the bias table is on another device")
+        starts = checked_starts(bias_table.shape[0], max_distance, False)
+    if _use_native("packed_causal_attention", q):
+        if dtype != torch.bfloat16 or qs[2] > 128:
+            raise TypeError(
+                "packed_causal_attention runs in bfloat16 with a head size "
+                f"of up to 128 on the GPU, got {dtype} and {qs[2]}")
+        if bias_table is not None and bias_table.dtype not in (
+                torch.bfloat16, torch.float32):
+            raise TypeError("the bias table has to be bfloat16 or float32 "
+                            f"on the GPU, got {bias_table.dtype}")
+        from . import native
+        return native.packed_causal_attention(q, k, v, packing, scale,
+                                              bias_table, starts)
+    return _packed_attention_plain(q, k, v, packing, scale, bias_table,
+                                   max_distance)
+
+
+def _refuse_packed_attention(q, k, v, packing):
+    """Says which of the arguments' conditions does not hold."""
     if not isinstance(packing, PackedSequences):
         raise TypeError("packing has to be a PackedSequences")
     if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape:
@@ -274,40 +315,10 @@ def packed_causal_attention(q, k, v, packing, scale=None, bias_table=None,
     if packing.total > rows:
         raise ValueError(f"the packing has {packing.total} rows, "
                          f"the tensors {rows}")
-    if len({t.device for t in (q, k, v)}) > 1:
+    if not (q.device == k.device == v.device):
         raise ValueError("q, k and v are on different devices")
-    if (q.is_cuda and q.dtype == torch.float32
-            and torch.is_autocast_enabled("cuda")):
-        q, k, v = (t.to(torch.bfloat16) for t in (q, k, v))
-    if not (q.is_floating_point() and q.dtype == k.dtype == v.dtype):
-        raise TypeError("q, k and v have to be of one floating type: "
-                        f"{q.dtype}, {k.dtype}, {v.dtype}")
-    scale = d ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < math.inf:
-        raise ValueError(f"scale has to be positive and finite, got {scale}")
-    starts = ()
-    if bias_table is not None:
-        if bias_table.dim() != 2 or bias_table.shape[1] != nhead:
-            raise ValueError(
-                f"the bias table is [num_buckets, {nhead}], got "
-                f"{tuple(bias_table.shape)}")
-        if bias_table.device != q.device:
-            raise ValueError("the bias table is on another device")
-        starts = checked_starts(bias_table.shape[0], max_distance, False)
-    if _use_native("packed_causal_attention", q):
-        if q.dtype != torch.bfloat16 or d > 128:
-            raise TypeError(
-                "packed_causal_attention runs in bfloat16 with a head size "
-                f"of up to 128 on the GPU, got {q.dtype} and {d}")
-        if bias_table is not None and bias_table.dtype not in (
-                torch.bfloat16, torch.float32):
-            raise TypeError("the bias table has to be bfloat16 or float32 "
-                            f"on the GPU, got {bias_table.dtype}")
-        from . import native
-        return native.packed_causal_attention(q, k, v, packing, scale,
-                                              bias_table, starts)
-    return _packed_attention_plain(q, k, v, packing, scale, bias_table,
-                                   max_distance)
+    raise TypeError("q, k and v have to be of one floating type: "
+                    f"{q.dtype}, {k.dtype}, {v.dtype}")
 
 
 def _packed_attention_plain(q, k, v, packing, scale, bias_table,

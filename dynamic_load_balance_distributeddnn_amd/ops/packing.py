@@ -127,14 +127,9 @@ class PackedSequences:
             # a synchronous copy: the lists are there for every stream
             both = torch.from_numpy(both).to(device)
             cut = len(lists[0][0])
-            self._lists[key] = (
-                (both[:cut], *lists[0][1:]), (both[cut:], *lists[1][1:]),
-                both, torch.cuda.current_stream(device))
-        queries, keys, both, made_on = self._lists[key]
-        now = torch.cuda.current_stream(device)
-        if now != made_on:
-            both.record_stream(now)
-        return queries, keys
+            self._lists[key] = ((both[:cut], *lists[0][1:]),
+                                (both[cut:], *lists[1][1:]))
+        return self._lists[key]
 
 
 @lru_cache(maxsize=64)
