@@ -330,12 +330,21 @@ __device__ inline int pa_bucket(const int* starts, int buckets, int n) {
   }
   return lo;
 }
+// A bias in the base-2 exponents that scores are held in.  Finite ones
+// beyond 1e37 (the types' lowest values, as masks) count as that: they
+// still drown any score, and stay finite.
 __device__ inline float pa_table(const PaBias& b, int bucket, int heads,
                                  int h) {
   const long at = (long)bucket * heads + h;
-  return b.is_bf16 ? (float)static_cast<const __bf16*>(b.table)[at]
-                   : static_cast<const float*>(b.table)[at];
+  const float x = b.is_bf16 ? (float)static_cast<const __bf16*>(b.table)[at]
+                            : static_cast<const float*>(b.table)[at];
+  const bool finite = x > -INFINITY && x < INFINITY;
+  const float y = x * PA_LOG2E;
+  return finite ? fminf(fmaxf(y, -1e37f), 1e37f) : y;
 }
+// Whether a tile's one bias can be added outside of the exponent's fma:
+// beyond, a score has to drown in it first.
+__device__ inline bool pa_moderate(float x) { return fabsf(x) <= 1e30f; }
 
 __device__ inline const __bf16* pa_at(const PaTensor& t, long row, int head) {
   return static_cast<const __bf16*>(t.p) + row * t.row + head * t.head;

@@ -58,25 +58,26 @@ __device__ inline void pa_bias_sums(const f32x16& ds, int n0,
   if (b >= 0 && b < buckets - 1 && (z == 63 || nb != b)) hist[b] += v;
 }
 
-// A query row's end: its gradient and delta.
-template <int DP, int W>
+// A query row's end: N x 32 elements of its gradient from 32 * t0 on, with
+// the first its delta.
+template <int W, int N>
 __device__ PA_INLINE void pa_bwd_q_end(const PaBwd& p, long first, int row,
                                        int len, int h,
-                                       const f32x16 (&acc)[DP / 32],
+                                       const f32x16 (&acc)[N], int t0,
                                        float delta) {
   if (row >= len) return;
   const int half = (threadIdx.x & 63) >> 5;
-  if (half == 0) p.delta[(long)h * p.T + first + row] = delta;
+  if (half == 0 && t0 == 0) p.delta[(long)h * p.T + first + row] = delta;
   __bf16* ob = static_cast<__bf16*>(p.dq) + ((first + row) * p.H + h) * p.D;
 #pragma unroll
-  for (int t = 0; t < DP / 32; ++t)
+  for (int t = 0; t < N; ++t)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       bf16x4 v;
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         v[e] = (__bf16)(acc[t][4 * g + e] * p.scale);
-      pa_store4<W>(ob, t * 32 + 8 * g + 4 * half, p.D, v);
+      pa_store4<W>(ob, (t0 + t) * 32 + 8 * g + 4 * half, p.D, v);
     }
 }
 
@@ -122,7 +123,7 @@ pa_bwd_q_kernel(const PaBwd p, const BiasArg bias) {
     return x;
   };
   auto near = [&](int k0) PA_INLINE {
-    return r0 - k0 - (PA_STEP - 1) < far_from;
+    return r0 - k0 - (PA_STEP - 1) < far_from || !pa_moderate(far_bias);
   };
 
   // a sequence's first rows, never in chunks: see above
@@ -159,7 +160,8 @@ pa_bwd_q_kernel(const PaBwd p, const BiasArg bias) {
       }
     }
   }
-  const float to2 = BIAS ? PA_LOG2E : p.scale * PA_LOG2E;
+  // scores are exponents of 2, as in the forward
+  const float mul = p.scale * PA_LOG2E;
 
   f32x16 acc[DT];
 #pragma unroll
@@ -191,25 +193,24 @@ pa_bwd_q_kernel(const PaBwd p, const BiasArg bias) {
 #pragma unroll
     for (int x = 0; x < KS; ++x)
       dp = pa_mfma(frags.rows(at + 4 * TILE, x), gf[x], dp);
+    float a = mul, off = -stat_l;
     if constexpr (BIAS) {
       if (near(k0)) {
         const float* w =
             s_win[buf] + wave * 32 + col + PA_STEP - 1;
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          s[r] = fmaf(s[r], p.scale,
-                      w[-(j * 32 + 8 * (r >> 2) + 4 * half + (r & 3))]);
+          s[r] = fmaf(s[r], mul,
+                      w[-(j * 32 + 8 * (r >> 2) + 4 * half + (r & 3))]) -
+                 stat_m;
+        a = 1.f;
       } else {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], p.scale, far_bias);
+        off = (far_bias - stat_m) - stat_l;
       }
     }
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const float e = BIAS ? fmaf(s[r] - stat_m, to2, -stat_l)
-                           : fmaf(s[r], to2, -stat_l);
-      s[r] = __builtin_amdgcn_exp2f(e) * (dp[r] - delta);
-    }
+    for (int r = 0; r < 16; ++r)
+      s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a, off)) * (dp[r] - delta);
     return s;
   };
   auto product = [&](bf16x8 w, int x) PA_INLINE {
@@ -304,52 +305,64 @@ pa_bwd_q_kernel(const PaBwd p, const BiasArg bias) {
     }
     return;
   }
-  pa_bwd_q_end<DP, W>(p, it.first, row, len, h, acc, delta + rest);
+  pa_bwd_q_end<W, DT>(p, it.first, row, len, h, acc, 0, delta + rest);
 }
 
-// Tiles in several chunks: the sums of their sums.
+// The sum of a tile's chunks: 32 elements of its rows, accumulators
+// 4 t .. 4 t + 3 of n.  Four chunks' loads together in flight, added in
+// their order.
+__device__ PA_INLINE f32x16 pa_joined(const PaWork& w, const PaJoin& j,
+                                      int heads, int h, int n, int t) {
+  f32x16 acc = pa_zero16();
+  for (int i0 = 0; i0 < j.n; i0 += 4) {
+    f32x4 x[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        x[i][g] = *pa_sums(w, j.slot + min(i0 + i, j.n - 1), heads, h, n,
+                           t * 4 + g);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (i0 + i >= j.n) break;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[r] += x[i][r >> 2][r & 3];
+    }
+  }
+  return acc;
+}
+
+// Tiles in several chunks; blockIdx.y: 32 elements of the rows.
 template <int DP, int W>
 __global__ void __launch_bounds__(PA_BLOCK)
 pa_bwd_q_join_kernel(const PaBwd p) {
-  const int DT = DP / 32;
   const int h = blockIdx.x % p.H;
   const PaJoin j = p.work_q.joins[blockIdx.x / p.H];
   const int in = (threadIdx.x >> 6) * 32 + (threadIdx.x & 31);
   float delta = pa_rows(p.work_q, j.slot, p.H, h, in)[0];
-  f32x16 acc[DT];
-#pragma unroll
-  for (int t = 0; t < DT; ++t) acc[t] = pa_zero16();
-  for (int i = 0; i < j.n; ++i) {
+  for (int i = 0; i < j.n; ++i)
     delta += pa_rows(p.work_q, j.slot + i, p.H, h, in)[1];
-#pragma unroll
-    for (int t = 0; t < DT; ++t)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4 x =
-            *pa_sums(p.work_q, j.slot + i, p.H, h, DT * 4, t * 4 + g);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[t][4 * g + e] += x[e];
-      }
-  }
-  pa_bwd_q_end<DP, W>(p, j.first, j.tile * PA_ROWS + in, j.len, h, acc,
-                      delta);
+  const f32x16 acc[1] = {
+      pa_joined(p.work_q, j, p.H, h, DP / 8, blockIdx.y)};
+  pa_bwd_q_end<W, 1>(p, j.first, j.tile * PA_ROWS + in, j.len, h, acc,
+                     blockIdx.y, delta);
 }
 
-// A key row's gradient.
-template <int DP, int W>
+// N x 32 elements of a key row's gradient from 32 * t0 on.
+template <int W, int N>
 __device__ PA_INLINE void pa_bwd_kv_end(const PaBwd& p, void* out, long row,
-                                        int hk, const f32x16 (&acc)[DP / 32],
-                                        float scale) {
+                                        int hk, const f32x16 (&acc)[N],
+                                        int t0, float scale) {
   const int half = (threadIdx.x & 63) >> 5;
   __bf16* to = static_cast<__bf16*>(out) + (row * (p.H / p.G) + hk) * p.D;
 #pragma unroll
-  for (int t = 0; t < DP / 32; ++t)
+  for (int t = 0; t < N; ++t)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       bf16x4 v;
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = (__bf16)(acc[t][4 * g + e] * scale);
-      pa_store4<W>(to, t * 32 + 8 * g + 4 * half, p.D, v);
+      pa_store4<W>(to, (t0 + t) * 32 + 8 * g + 4 * half, p.D, v);
     }
 }
 
@@ -394,8 +407,8 @@ pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
     far_from = bias.starts[bias.buckets - 1];
     __syncthreads();
   }
-  auto near = [&](int q0) PA_INLINE {
-    return q0 - c0 - (PA_ROWS - 1) < far_from;
+  auto near = [&](int q0, float far) PA_INLINE {
+    return q0 - c0 - (PA_ROWS - 1) < far_from || !pa_moderate(far);
   };
   auto window = [&](int q0, int h) PA_INLINE {
     float x = 0.f;
@@ -414,7 +427,8 @@ pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
     for (int s = 0; s < KS; ++s)
       kf[s] = pa_load8<W>(kb, s * 16 + half * 8, p.D);
   }
-  const float to2 = BIAS ? PA_LOG2E : p.scale * PA_LOG2E;
+  // scores are exponents of 2, as in the forward
+  const float mul = p.scale * PA_LOG2E;
 
   f32x16 dk[DT], dv[DT];
 #pragma unroll
@@ -428,6 +442,12 @@ pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
     gs.base = pa_at(p.go, it.first, h);
     qs.start(q0, s_q[buf]);
     gs.start(q0, s_g[buf]);
+    bool each = false;
+    if constexpr (BIAS) {
+      next_far = pa_table(bias, bias.buckets - 1, p.H, h);
+      each = near(q0, next_far);
+      if (each) win = window(q0, h);
+    }
     if (threadIdx.x < ROWS) {
       // rows behind the sequence: weights of exp2(-inf)
       st_l = INFINITY;
@@ -438,14 +458,14 @@ pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
         if constexpr (BIAS) {
           st_m = p.stats[2 * at];
           st_l = p.stats[2 * at + 1];
+          // a tile of one bias: all in one
+          if (!each) st_l -= next_far - st_m;
         } else {
           st_l = p.stats[at];
         }
         st_d = p.delta[at];
       }
     }
-    if (BIAS && near(q0)) win = window(q0, h);
-    if constexpr (BIAS) next_far = pa_table(bias, bias.buckets - 1, p.H, h);
   };
   auto arrive = [&](int q0, int buf) PA_INLINE {
     if (threadIdx.x < ROWS) {
@@ -453,7 +473,8 @@ pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
       s_delta[buf][threadIdx.x] = st_d;
       if (BIAS) s_m[buf][threadIdx.x] = st_m;
     }
-    if (BIAS && near(q0) && threadIdx.x < 192) s_win[buf][threadIdx.x] = win;
+    if (BIAS && near(q0, next_far) && threadIdx.x < 192)
+      s_win[buf][threadIdx.x] = win;
     far_bias = next_far;
     qs.arrive(q0, s_q[buf]);
     gs.arrive(q0, s_g[buf]);
@@ -474,16 +495,19 @@ pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
     for (int x = 0; x < KS; ++x)
       dp = pa_mfma(frags.rows(2 * TILE * 2, x),
                    vfrags.rows(4 * TILE * 2, x), dp);
-    if constexpr (BIAS) {
-      if (near(q0)) {
-        const float* w = s_win[buf] + PA_ROWS - 1 - wave * 32 - col;
+    bool each = false;
+    if constexpr (BIAS) each = near(q0, far_bias);
+    const float a = each ? 1.f : mul;
+    if (each) {
+      const float* w = s_win[BIAS ? buf : 0] + PA_ROWS - 1 - wave * 32 - col;
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          s[r] = fmaf(s[r], p.scale,
-                      w[8 * (r >> 2) + 4 * half + (r & 3)]);
-      } else {
+      for (int g = 0; g < 4; ++g) {
+        const int at = 8 * g + 4 * half;
+        const f32x4 mv = *reinterpret_cast<const f32x4*>(
+            &s_m[buf][BIAS ? at : 0]);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], p.scale, far_bias);
+        for (int e = 0; e < 4; ++e)
+          s[4 * g + e] = fmaf(s[4 * g + e], mul, w[at + e]) - mv[e];
       }
     }
 #pragma unroll
@@ -491,15 +515,10 @@ pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
       const int at = 8 * g + 4 * half;
       const f32x4 lv = *reinterpret_cast<const f32x4*>(&s_l[buf][at]);
       const f32x4 ev = *reinterpret_cast<const f32x4*>(&s_delta[buf][at]);
-      f32x4 mv = {0.f, 0.f, 0.f, 0.f};
-      if constexpr (BIAS)
-        mv = *reinterpret_cast<const f32x4*>(&s_m[buf][at]);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int r = 4 * g + e;
-        s[r] = __builtin_amdgcn_exp2f(BIAS
-                                          ? fmaf(s[r] - mv[e], to2, -lv[e])
-                                          : fmaf(s[r], to2, -lv[e]));
+        s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a, -lv[e]));
         dp[r] = s[r] * (dp[r] - ev[e]);
       }
     }
@@ -660,36 +679,25 @@ pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
   }
   if (key < len) {
     const long at = (long)it.first + key;
-    pa_bwd_kv_end<DP, W>(p, p.dk, at, hk, dk, p.scale);
-    pa_bwd_kv_end<DP, W>(p, p.dv, at, hk, dv, 1.f);
+    pa_bwd_kv_end<W, DT>(p, p.dk, at, hk, dk, 0, p.scale);
+    pa_bwd_kv_end<W, DT>(p, p.dv, at, hk, dv, 0, 1.f);
   }
 }
 
-// Tiles in several chunks: the sums of their sums; blockIdx.y: dK or dV.
+// Tiles in several chunks; blockIdx.y: 32 elements of dK's rows or dV's.
 template <int DP, int W>
 __global__ void __launch_bounds__(PA_BLOCK)
 pa_bwd_kv_join_kernel(const PaBwd p) {
-  const int DT = DP / 32;
   const int kvh = p.H / p.G, hk = blockIdx.x % kvh;
   const PaJoin j = p.work_kv.joins[blockIdx.x / kvh];
   const int key = j.tile * PA_ROWS + (threadIdx.x >> 6) * 32 +
                   (threadIdx.x & 31);
-  f32x16 acc[DT];
-#pragma unroll
-  for (int t = 0; t < DT; ++t) acc[t] = pa_zero16();
-  for (int i = 0; i < j.n; ++i)
-#pragma unroll
-    for (int t = 0; t < DT; ++t)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4 x = *pa_sums(p.work_kv, j.slot + i, kvh, hk, DT * 8,
-                                 t * 8 + 4 * (int)blockIdx.y + g);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[t][4 * g + e] += x[e];
-      }
+  const f32x16 acc[1] = {
+      pa_joined(p.work_kv, j, kvh, hk, DP / 4, blockIdx.y)};
+  const bool v = blockIdx.y & 1;
   if (key < j.len)
-    pa_bwd_kv_end<DP, W>(p, blockIdx.y ? p.dv : p.dk, (long)j.first + key, hk,
-                         acc, blockIdx.y ? 1.f : p.scale);
+    pa_bwd_kv_end<W, 1>(p, v ? p.dv : p.dk, (long)j.first + key, hk, acc,
+                        blockIdx.y >> 1, v ? 1.f : p.scale);
 }
 
 // dtable[b, h] from the chunks' partial sums; a workgroup a head, a wave a
@@ -727,9 +735,10 @@ static void pa_bwd_go(const PaBwd& p, const PaBias* bias,
                       hipStream_t stream) {
   const unsigned H = p.H, kvh = p.H / p.G;
   const dim3 block(PA_BLOCK);
-  const dim3 grid(p.work_q.n_chunks * H), joins(p.work_q.n_joins * H);
+  const dim3 grid(p.work_q.n_chunks * H);
+  const dim3 joins(p.work_q.n_joins * H, DP / 32);
   const dim3 grid_kv(p.work_kv.n_chunks * kvh);
-  const dim3 joins_kv(p.work_kv.n_joins * kvh, 2);
+  const dim3 joins_kv(p.work_kv.n_joins * kvh, DP / 16);
   if (bias)
     hipLaunchKernelGGL((pa_bwd_q_kernel<DP, W, true, PaBias>), grid, block, 0,
                        stream, p, *bias);

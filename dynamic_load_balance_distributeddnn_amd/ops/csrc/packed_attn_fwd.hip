@@ -12,11 +12,12 @@
 // to several workgroups is put together by a second kernel.
 #include "packed_attn.h"
 
-// A row's end: its output and its statistics.
-template <int DP, int W, bool BIAS>
+// A row's end: N x 32 elements of its output from 32 * t0 on, with the
+// first its statistics.
+template <int W, bool BIAS, int N>
 __device__ PA_INLINE void pa_fwd_end(const PaFwd& p, long first, int row,
-                                     int len, int h, f32x16 (&acc)[DP / 32],
-                                     float m, float l) {
+                                     int len, int h, const f32x16 (&acc)[N],
+                                     int t0, float m, float l) {
   if (row >= len) return;
   const int half = (threadIdx.x & 63) >> 5;
   // no weight anywhere (a bias of -inf on all a row sees): zeros, and
@@ -24,15 +25,15 @@ __device__ PA_INLINE void pa_fwd_end(const PaFwd& p, long first, int row,
   const float inv = l == 0.f ? 0.f : 1.f / l;
   __bf16* ob = static_cast<__bf16*>(p.o) + ((first + row) * p.H + h) * p.D;
 #pragma unroll
-  for (int t = 0; t < DP / 32; ++t)
+  for (int t = 0; t < N; ++t)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       bf16x4 v;
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = (__bf16)(acc[t][4 * g + e] * inv);
-      pa_store4<W>(ob, t * 32 + 8 * g + 4 * half, p.D, v);
+      pa_store4<W>(ob, (t0 + t) * 32 + 8 * g + 4 * half, p.D, v);
     }
-  if (half == 0) {
+  if (half == 0 && t0 == 0) {
     const long at = (long)h * p.T + first + row;
     const float lg = l == 0.f ? INFINITY : __builtin_amdgcn_logf(l);
     const float top = m == -INFINITY ? 0.f : m;
@@ -40,7 +41,7 @@ __device__ PA_INLINE void pa_fwd_end(const PaFwd& p, long first, int row,
       p.stats[2 * at] = top;
       p.stats[2 * at + 1] = lg;
     } else {
-      p.stats[at] = top * (p.scale * PA_LOG2E) + lg;
+      p.stats[at] = top + lg;
     }
   }
 }
@@ -87,7 +88,7 @@ pa_fwd_kernel(const PaFwd p, const BiasArg bias) {
     return x;
   };
   auto near = [&](int k0) PA_INLINE {
-    return r0 - k0 - (PA_STEP - 1) < far_from;
+    return r0 - k0 - (PA_STEP - 1) < far_from || !pa_moderate(far_bias);
   };
 
   bf16x8 qf[KS];
@@ -101,9 +102,12 @@ pa_fwd_kernel(const PaFwd p, const BiasArg bias) {
   f32x16 acc[DT];
 #pragma unroll
   for (int t = 0; t < DT; ++t) acc[t] = pa_zero16();
-  float m = -INFINITY;   // running maximum: of q.k, with bias of S
+  // Scores are exponents of 2, a s + b: in tiles of one bias (or none) s is
+  // q.k as the product leaves it, elsewhere the sum, with a = 1, b = 0.
+  float m = -INFINITY;   // running maximum
   float l = 0.f;         // this half's part of the sum
-  const float to2 = BIAS ? PA_LOG2E : p.scale * PA_LOG2E;
+  const float mul = p.scale * PA_LOG2E;
+  float a = mul, b = far_bias;
 
   PaStage<DP, W> ks{pa_at(p.k, it.first, h / p.G), p.k.row, len, p.D};
   PaStage<DP, W> vs{pa_at(p.v, it.first, h / p.G), p.v.row, len, p.D};
@@ -139,20 +143,17 @@ pa_fwd_kernel(const PaFwd p, const BiasArg bias) {
                        qf[x], s[j]);
     }
     if constexpr (BIAS) {
-      if (near(k0)) {
+      const bool each = near(k0);
+      a = each ? 1.f : mul;
+      b = each ? 0.f : far_bias;
+      if (each) {
         const float* w = s_win[buf] + wave * 32 + col + (PA_STEP - 1);
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int r = 0; r < 16; ++r)
-            s[j][r] = fmaf(s[j][r], p.scale,
+            s[j][r] = fmaf(s[j][r], mul,
                            w[-(j * 32 + 8 * (r >> 2) + 4 * half + (r & 3))]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            s[j][r] = fmaf(s[j][r], p.scale, far_bias);
       }
     }
   };
@@ -162,21 +163,19 @@ pa_fwd_kernel(const PaFwd p, const BiasArg bias) {
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, s[j][r]);
-    return fmaxf(m, pa_half_max(top));
+    return fmaxf(m, fmaf(pa_half_max(top), a, b));
   };
   auto weights = [&](f32x16 (&s)[2], float ref) PA_INLINE {
-    const float off = ref * to2;
+    const float off = b - ref;
+    float sum[4] = {};
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        // with a bias the scores may stand at the type's lowest value: the
-        // difference is taken before the change of base
-        const float e = BIAS ? (s[j][r] - ref) * to2
-                             : fmaf(s[j][r], to2, -off);
-        s[j][r] = __builtin_amdgcn_exp2f(e);
-        l += s[j][r];
+        s[j][r] = __builtin_amdgcn_exp2f(fmaf(s[j][r], a, off));
+        sum[r & 3] += s[j][r];
       }
+    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
   };
   auto values = [&](const f32x16 (&s)[2]) PA_INLINE {
 #pragma unroll
@@ -215,7 +214,7 @@ pa_fwd_kernel(const PaFwd p, const BiasArg bias) {
           if (j * 32 + 8 * (r >> 2) + (r & 3) > lim) s[j][r] = -INFINITY;
       const float top = maximum(s);
       const float ref = top == -INFINITY ? 0.f : top;
-      const float f = __builtin_amdgcn_exp2f((m - ref) * to2);
+      const float f = __builtin_amdgcn_exp2f(m - ref);
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -240,7 +239,7 @@ pa_fwd_kernel(const PaFwd p, const BiasArg bias) {
     frags = lanes.fresh(buf * TILE * 2);
     f32x16 s[2];
     scores(s, k0, buf);
-    if (__any((maximum(s) - m) * to2 > 16.f)) return false;
+    if (__any(maximum(s) - m > 16.f)) return false;
     weights(s, m == -INFINITY ? 0.f : m);
     values(s);
     if (more) arrive(k0 + PA_STEP, buf ^ 1);
@@ -270,49 +269,64 @@ pa_fwd_kernel(const PaFwd p, const BiasArg bias) {
     }
     return;
   }
-  pa_fwd_end<DP, W, BIAS>(p, it.first, row, len, h, acc, m, l);
+  pa_fwd_end<W, BIAS, DT>(p, it.first, row, len, h, acc, 0, m, l);
 }
 
 // Tiles in several chunks: with the largest maximum of a row,
-// O = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i.
+// O = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i; blockIdx.y: 32
+// elements of the rows.
 template <int DP, int W, bool BIAS>
 __global__ void __launch_bounds__(PA_BLOCK)
 pa_fwd_join_kernel(const PaFwd p) {
   const int DT = DP / 32;
-  const int h = blockIdx.x % p.H;
+  const int h = blockIdx.x % p.H, t = blockIdx.y;
   const PaJoin j = p.work.joins[blockIdx.x / p.H];
   const int in = (threadIdx.x >> 6) * 32 + (threadIdx.x & 31);
-  const float to2 = BIAS ? PA_LOG2E : p.scale * PA_LOG2E;
   float m = -INFINITY, l = 0.f;
-  for (int i = 0; i < j.n; ++i)
-    m = fmaxf(m, pa_rows(p.work, j.slot + i, p.H, h, in)[0]);
-  const float ref = m == -INFINITY ? 0.f : m;
-  f32x16 acc[DT];
+  f32x16 acc[1] = {pa_zero16()};
+  // four chunks at a time, their loads together in flight; the running
+  // maximum as in the tiles
+  for (int i0 = 0; i0 < j.n; i0 += 4) {
+    f32x4 x[4][4];
+    float mi[4], li[4], top = m;
 #pragma unroll
-  for (int t = 0; t < DT; ++t) acc[t] = pa_zero16();
-  for (int i = 0; i < j.n; ++i) {
-    const float* from = pa_rows(p.work, j.slot + i, p.H, h, in);
-    const float f = __builtin_amdgcn_exp2f((from[0] - ref) * to2);
-    l += f * from[1];
+    for (int i = 0; i < 4; ++i) {
+      const int slot = j.slot + min(i0 + i, j.n - 1);
+      const float* from = pa_rows(p.work, slot, p.H, h, in);
+      const bool there = i0 + i < j.n;
+      mi[i] = there ? from[0] : -INFINITY;
+      li[i] = there ? from[1] : 0.f;
 #pragma unroll
-    for (int t = 0; t < DT; ++t)
+      for (int g = 0; g < 4; ++g)
+        x[i][g] = *pa_sums(p.work, slot, p.H, h, DT * 4, t * 4 + g);
+    }
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4 x =
-            *pa_sums(p.work, j.slot + i, p.H, h, DT * 4, t * 4 + g);
+    for (int i = 0; i < 4; ++i) top = fmaxf(top, mi[i]);
+    const float ref = top == -INFINITY ? 0.f : top;
+    const float f = __builtin_amdgcn_exp2f(m - ref);
+    m = top;
+    l *= f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[t][4 * g + e] += f * x[e];
-      }
+    for (int r = 0; r < 16; ++r) acc[0][r] *= f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (i0 + i >= j.n) break;
+      const float fi = __builtin_amdgcn_exp2f(mi[i] - ref);
+      l += fi * li[i];
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        acc[0][r] = fmaf(fi, x[i][r >> 2][r & 3], acc[0][r]);
+    }
   }
-  pa_fwd_end<DP, W, BIAS>(p, j.first, j.tile * PA_ROWS + in, j.len, h, acc, m,
-                          l);
+  pa_fwd_end<W, BIAS, 1>(p, j.first, j.tile * PA_ROWS + in, j.len, h, acc, t,
+                         m, l);
 }
 
 template <int DP, int W>
 static void pa_fwd_go(const PaFwd& p, const PaBias* bias,
                       hipStream_t stream) {
   const dim3 grid((unsigned)p.work.n_chunks * p.H), block(PA_BLOCK);
-  const dim3 joins((unsigned)p.work.n_joins * p.H);
+  const dim3 joins((unsigned)p.work.n_joins * p.H, DP / 32);
   if (bias) {
     hipLaunchKernelGGL((pa_fwd_kernel<DP, W, true, PaBias>), grid, block, 0,
                        stream, p, *bias);
