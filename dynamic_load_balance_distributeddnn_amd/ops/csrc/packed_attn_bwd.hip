@@ -24,38 +24,87 @@
 // their one or two key tiles beforehand.
 #include "packed_attn.h"
 
-// Sums of the table's gradient over one 32 x 32 block of dS (queries x
-// keys, the result layout; masked pairs 0): lane l first collects the
-// diagonals l & 31 and (l & 31) - 32, then neighbouring diagonals of one
-// bucket are added up lane by lane, in a fixed order.  `n0` is the
-// distance of diagonal 0.  The last bucket is left out: a row's dS sum to
-// 0, so it is minus the sum of the others.
-__device__ inline void pa_bias_sums(const f32x16& ds, int n0,
-                                    const int* starts, int buckets,
-                                    float* hist, int lane) {
-  const int x = lane & 31, half = lane >> 5;
-  float hi = 0.f, lo = 0.f;
-#pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    const int i = 8 * (r >> 2) + 4 * half + (r & 3);
-    const float v = __shfl(ds[r], ((i - x) & 31) + 32 * half, 64);
-    if (x <= i) hi += v; else lo += v;
+// ---- The table's gradient: sums of dS along its diagonals, then of the
+// diagonals of a bucket, all in a fixed order.  The last bucket is left
+// out: a row's dS sum to 0, so it is minus the sum of the others.
+#define PA_DISTANCES 512
+
+// Lane l gets the value of lane (l + N) & 31 of its half.
+template <int N>
+__device__ inline float pa_rotate(float v) {
+  return N == 0 ? v
+                : __builtin_bit_cast(float, __builtin_amdgcn_ds_swizzle(
+                                                __builtin_bit_cast(int, v),
+                                                0xc000 | (N << 5)));
+}
+
+// Diagonals of one 32 x 32 block of dS (queries x keys, the result layout;
+// masked pairs 0): register r of half h, query i = c + 4 h, rotated by c
+// leaves in lane x the distance 4 h - x, or 32 more where it wrapped.
+__device__ PA_INLINE void pa_diagonals(const f32x16& ds, float& a, float& b,
+                                       int x) {
+  a = b = 0.f;
+#define PA_DIAGONAL(R)                                   \
+  {                                                      \
+    constexpr int c = 8 * (R >> 2) + (R & 3);            \
+    const float v = pa_rotate<c>(ds[R]);                 \
+    if (x + c < 32) a += v; else b += v;                 \
   }
-  hi = pa_half_sum(hi);
-  lo = pa_half_sum(lo);
-  float v = half ? lo : hi;
-  const int z = lane ^ 32;  // diagonals in the order of their distance
-  const int n = n0 - 32 + z;
-  const int b = n < 0 ? -1 : pa_bucket(starts, buckets, n);
+  PA_DIAGONAL(0) PA_DIAGONAL(1) PA_DIAGONAL(2) PA_DIAGONAL(3)
+  PA_DIAGONAL(4) PA_DIAGONAL(5) PA_DIAGONAL(6) PA_DIAGONAL(7)
+  PA_DIAGONAL(8) PA_DIAGONAL(9) PA_DIAGONAL(10) PA_DIAGONAL(11)
+  PA_DIAGONAL(12) PA_DIAGONAL(13) PA_DIAGONAL(14) PA_DIAGONAL(15)
+#undef PA_DIAGONAL
+}
+
+// Adds them to the wave's sums by distance; `n0` is the distance of query
+// 0 and key 0 of the block.  The halves one after the other: no two lanes
+// of an addition meet.
+__device__ PA_INLINE void pa_add_diagonals(const f32x16& ds, int n0,
+                                           int far_from, float* sums,
+                                           int lane) {
+  const int x = lane & 31;
+  float a, b;
+  pa_diagonals(ds, a, b, x);
 #pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int src = ((z - off) & 63) ^ 32;
-    const float pv = __shfl(v, src, 64);
-    const int pb = __shfl(b, src, 64);
-    if (z >= off && pb == b) v += pv;
+  for (int h = 0; h < 2; ++h) {
+    const int n = n0 + 4 * h - x;
+    if ((lane >> 5) == h) {
+      if (n >= 0 && n < far_from)
+        __hip_atomic_fetch_add(sums + n, a, __ATOMIC_RELAXED,
+                               __HIP_MEMORY_SCOPE_WORKGROUP);
+      if (n + 32 >= 0 && n + 32 < far_from)
+        __hip_atomic_fetch_add(sums + n + 32, b, __ATOMIC_RELAXED,
+                               __HIP_MEMORY_SCOPE_WORKGROUP);
+    }
   }
-  const int nb = __shfl(b, ((z + 1) & 63) ^ 32, 64);
-  if (b >= 0 && b < buckets - 1 && (z == 63 || nb != b)) hist[b] += v;
+}
+
+// The same where there are too many distances for LDS: neighbouring
+// diagonals of one bucket are added up lane by lane first.
+__device__ PA_INLINE void pa_add_buckets(const f32x16& ds, int n0,
+                                         const int* starts, int buckets,
+                                         float* sums, int lane) {
+  float part[2];
+  pa_diagonals(ds, part[0], part[1], lane & 31);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    // in the order of their distances: half by half, lanes downwards
+    const int n = n0 + 4 * (lane >> 5) - (lane & 31) + 32 * i;
+    const int z = 31 - (lane & 31);
+    float v = part[i];
+    const int b = n < 0 ? -1 : pa_bucket(starts, buckets, n);
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const float pv = __shfl_down(v, off, 64);
+      const int pb = __shfl_down(b, off, 64);
+      if (z >= off && pb == b) v += pv;
+    }
+    const int nb = __shfl_up(b, 1, 64);
+    const bool last = b >= 0 && b < buckets - 1 && (z == 31 || nb != b);
+    if (last && lane < 32) sums[b] += v;
+    if (last && lane >= 32) sums[b] += v;
+  }
 }
 
 // A query row's end: N x 32 elements of its gradient from 32 * t0 on, with
@@ -381,7 +430,8 @@ pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
   __shared__ __attribute__((aligned(16))) float s_m[2][BIAS ? ROWS : 4];
   __shared__ float s_win[BIAS ? 2 : 1][BIAS ? 192 : 1];
   __shared__ int s_start[BIAS ? PA_MAXBUCKETS : 1];
-  __shared__ float s_hist[BIAS ? 4 : 1][BIAS ? PA_MAXBUCKETS : 1];
+  // sums of each wave by distance, or by bucket where far_from is larger
+  __shared__ float s_sums[BIAS ? 4 : 1][BIAS ? PA_DISTANCES : 1];
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -400,10 +450,10 @@ pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
   float far_bias = 0.f, next_far = 0.f;  // of this and the next step
   int far_from = 0;
   if constexpr (BIAS) {
-    for (int b = threadIdx.x; b < bias.buckets; b += PA_BLOCK) {
+    for (int b = threadIdx.x; b < bias.buckets; b += PA_BLOCK)
       s_start[b] = bias.starts[b];
-      for (int w = 0; w < 4; ++w) s_hist[w][b] = 0.f;
-    }
+    for (int i = threadIdx.x; i < 4 * PA_DISTANCES; i += PA_BLOCK)
+      s_sums[0][i] = 0.f;
     far_from = bias.starts[bias.buckets - 1];
     __syncthreads();
   }
@@ -529,7 +579,11 @@ pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
       if (p.part && n0 - 31 < far_from) {
         f32x16 mine = dp;
         if (key >= len) mine = pa_zero16();
-        pa_bias_sums(mine, n0, s_start, bias.buckets, s_hist[wave], lane);
+        if (far_from <= PA_DISTANCES)
+          pa_add_diagonals(mine, n0, far_from, s_sums[wave], lane);
+        else
+          pa_add_buckets(mine, n0, s_start, bias.buckets, s_sums[wave],
+                         lane);
       }
     }
   };
@@ -644,11 +698,25 @@ pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
       if (p.part) {
         __syncthreads();
         float* out = p.part + (chunk * p.H + h0 + head) * bias.buckets;
-        for (int b = threadIdx.x; b < bias.buckets; b += PA_BLOCK) {
-          out[b] = (s_hist[0][b] + s_hist[1][b]) +
-                   (s_hist[2][b] + s_hist[3][b]);
-          for (int w = 0; w < 4; ++w) s_hist[w][b] = 0.f;
+        const bool by_distance = far_from <= PA_DISTANCES;
+        // eight threads a bucket
+        for (int b = threadIdx.x >> 3; b < bias.buckets; b += PA_BLOCK / 8) {
+          const int from = by_distance ? s_start[b] : b;
+          const int to = b == bias.buckets - 1 ? from
+                         : by_distance         ? s_start[b + 1]
+                                               : b + 1;
+          float v = 0.f;
+          for (int n = from + (threadIdx.x & 7); n < to; n += 8)
+            v += (s_sums[0][n] + s_sums[1][n]) +
+                 (s_sums[2][n] + s_sums[3][n]);
+          v += __shfl_xor(v, 1, 64);
+          v += __shfl_xor(v, 2, 64);
+          v += __shfl_xor(v, 4, 64);
+          if ((threadIdx.x & 7) == 0) out[b] = v;
         }
+        __syncthreads();
+        for (int i = threadIdx.x; i < 4 * PA_DISTANCES; i += PA_BLOCK)
+          s_sums[0][i] = 0.f;
         __syncthreads();
       }
     }
