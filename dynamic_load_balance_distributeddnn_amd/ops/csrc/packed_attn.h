@@ -330,14 +330,18 @@ __device__ inline int pa_bucket(const int* starts, int buckets, int n) {
   }
   return lo;
 }
+// A table's entry as it stands in memory.
+__device__ inline unsigned pa_table(const PaBias& b, int bucket, int heads,
+                                    int h) {
+  const long at = (long)bucket * heads + h;
+  if (b.is_bf16) return static_cast<const unsigned short*>(b.table)[at];
+  return static_cast<const unsigned*>(b.table)[at];
+}
 // A bias in the base-2 exponents that scores are held in.  Finite ones
 // beyond 1e37 (the types' lowest values, as masks) count as that: they
 // still drown any score, and stay finite.
-__device__ inline float pa_table(const PaBias& b, int bucket, int heads,
-                                 int h) {
-  const long at = (long)bucket * heads + h;
-  const float x = b.is_bf16 ? (float)static_cast<const __bf16*>(b.table)[at]
-                            : static_cast<const float*>(b.table)[at];
+__device__ inline float pa_bias(unsigned entry, int is_bf16) {
+  const float x = __uint_as_float(is_bf16 ? entry << 16 : entry);
   const bool finite = x > -INFINITY && x < INFINITY;
   const float y = x * PA_LOG2E;
   return finite ? fminf(fmaxf(y, -1e37f), 1e37f) : y;

@@ -28,6 +28,7 @@
 // diagonals of a bucket, all in a fixed order.  The last bucket is left
 // out: a row's dS sum to 0, so it is minus the sum of the others.
 #define PA_DISTANCES 512
+#define PA_FARHEADS 32
 
 // Lane l gets the value of lane (l + N) & 31 of its half.
 template <int N>
@@ -131,7 +132,7 @@ __device__ PA_INLINE void pa_bwd_q_end(const PaBwd& p, long first, int row,
 }
 
 template <int DP, int W, bool BIAS, typename BiasArg>
-__global__ void __launch_bounds__(PA_BLOCK, 2)
+__global__ void __launch_bounds__(PA_BLOCK, DP == 64 && BIAS ? 3 : 2)
 pa_bwd_q_kernel(const PaBwd p, const BiasArg bias) {
   const int KS = DP / 16, DT = DP / 32;
   const int TILE = PA_STEP * DP;
@@ -156,7 +157,7 @@ pa_bwd_q_kernel(const PaBwd p, const BiasArg bias) {
   int far_from = 0;
   if constexpr (BIAS) {
     for (int b = threadIdx.x; b < bias.buckets; b += PA_BLOCK) {
-      s_tab[b] = pa_table(bias, b, p.H, h);
+      s_tab[b] = pa_bias(pa_table(bias, b, p.H, h), bias.is_bf16);
       s_start[b] = bias.starts[b];
     }
     __syncthreads();
@@ -430,6 +431,9 @@ pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
   __shared__ __attribute__((aligned(16))) float s_m[2][BIAS ? ROWS : 4];
   __shared__ float s_win[BIAS ? 2 : 1][BIAS ? 192 : 1];
   __shared__ int s_start[BIAS ? PA_MAXBUCKETS : 1];
+  // far bias of each head of the group, buckets by distance
+  __shared__ float s_far[BIAS ? PA_FARHEADS : 1];
+  __shared__ unsigned char s_bucket[BIAS ? PA_DISTANCES : 1];
   // sums of each wave by distance, or by bucket where far_from is larger
   __shared__ float s_sums[BIAS ? 4 : 1][BIAS ? PA_DISTANCES : 1];
 
@@ -454,18 +458,28 @@ pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
       s_start[b] = bias.starts[b];
     for (int i = threadIdx.x; i < 4 * PA_DISTANCES; i += PA_BLOCK)
       s_sums[0][i] = 0.f;
+    for (int x = threadIdx.x; x < min(p.G, PA_FARHEADS); x += PA_BLOCK)
+      s_far[x] = pa_bias(pa_table(bias, bias.buckets - 1, p.H, hk * p.G + x),
+                         bias.is_bf16);
     far_from = bias.starts[bias.buckets - 1];
     __syncthreads();
+    for (int n = threadIdx.x; n < PA_DISTANCES; n += PA_BLOCK)
+      s_bucket[n] = pa_bucket(s_start, bias.buckets, n);
+    __syncthreads();
   }
+  // Nothing that a step asks memory for is looked at before the step ends:
+  // a wait for it would be a wait for the tiles asked for before.
   auto near = [&](int q0, float far) PA_INLINE {
     return q0 - c0 - (PA_ROWS - 1) < far_from || !pa_moderate(far);
   };
   auto window = [&](int q0, int h) PA_INLINE {
-    float x = 0.f;
+    unsigned x = 0;
     if constexpr (BIAS) {
-      const int n = q0 - c0 - (PA_ROWS - 1) + (int)threadIdx.x;
-      if (n >= 0)
-        x = pa_table(bias, pa_bucket(s_start, bias.buckets, n), p.H, h);
+      const int n = max(q0 - c0 - (PA_ROWS - 1) + (int)threadIdx.x, 0);
+      const int b = n >= far_from      ? bias.buckets - 1
+                    : n < PA_DISTANCES ? s_bucket[n]
+                                       : pa_bucket(s_start, bias.buckets, n);
+      x = pa_table(bias, b, p.H, h);
     }
     return x;
   };
@@ -486,17 +500,20 @@ pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
 
   PaStage<DP, W, ROWS> qs{nullptr, p.q.row, len, p.D};
   PaStage<DP, W, ROWS> gs{nullptr, p.go.row, len, p.D};
-  float win = 0.f, st_l = 0.f, st_d = 0.f, st_m = 0.f;
+  unsigned win = 0;
+  float st_l = 0.f, st_d = 0.f, st_m = 0.f;
   auto start = [&](int q0, int h, int buf) PA_INLINE {
     qs.base = pa_at(p.q, it.first, h);
     gs.base = pa_at(p.go, it.first, h);
     qs.start(q0, s_q[buf]);
     gs.start(q0, s_g[buf]);
-    bool each = false;
     if constexpr (BIAS) {
-      next_far = pa_table(bias, bias.buckets - 1, p.H, h);
-      each = near(q0, next_far);
-      if (each) win = window(q0, h);
+      const int g = h - hk * p.G;
+      next_far = g < PA_FARHEADS
+                     ? s_far[g]
+                     : pa_bias(pa_table(bias, bias.buckets - 1, p.H, h),
+                               bias.is_bf16);
+      if (near(q0, next_far)) win = window(q0, h);
     }
     if (threadIdx.x < ROWS) {
       // rows behind the sequence: weights of exp2(-inf)
@@ -508,8 +525,6 @@ pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
         if constexpr (BIAS) {
           st_m = p.stats[2 * at];
           st_l = p.stats[2 * at + 1];
-          // a tile of one bias: all in one
-          if (!each) st_l -= next_far - st_m;
         } else {
           st_l = p.stats[at];
         }
@@ -518,16 +533,21 @@ pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
     }
   };
   auto arrive = [&](int q0, int buf) PA_INLINE {
+    qs.arrive(q0, s_q[buf]);
+    gs.arrive(q0, s_g[buf]);
+    const bool each = BIAS && near(q0, next_far);
     if (threadIdx.x < ROWS) {
+      // a tile of one bias: all in one
+      if (BIAS && !each) st_l -= next_far - st_m;
       s_l[buf][threadIdx.x] = st_l;
       s_delta[buf][threadIdx.x] = st_d;
       if (BIAS) s_m[buf][threadIdx.x] = st_m;
     }
-    if (BIAS && near(q0, next_far) && threadIdx.x < 192)
-      s_win[buf][threadIdx.x] = win;
+    if constexpr (BIAS) {
+      if (each && threadIdx.x < 192)
+        s_win[buf][threadIdx.x] = pa_bias(win, bias.is_bf16);
+    }
     far_bias = next_far;
-    qs.arrive(q0, s_q[buf]);
-    gs.arrive(q0, s_g[buf]);
     __syncthreads();
   };
 

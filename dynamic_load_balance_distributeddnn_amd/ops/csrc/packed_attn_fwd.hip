@@ -71,7 +71,7 @@ pa_fwd_kernel(const PaFwd p, const BiasArg bias) {
   int far_from = 0;
   if constexpr (BIAS) {
     for (int b = threadIdx.x; b < bias.buckets; b += PA_BLOCK) {
-      s_tab[b] = pa_table(bias, b, p.H, h);
+      s_tab[b] = pa_bias(pa_table(bias, b, p.H, h), bias.is_bf16);
       s_start[b] = bias.starts[b];
     }
     __syncthreads();
