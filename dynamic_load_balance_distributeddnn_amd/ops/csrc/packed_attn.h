@@ -226,10 +226,21 @@ template <int DP, int W, int ROWS = PA_STEP>
 struct PaStage {
   static const int LANES = DP * 2 / W;          // of a row
   static const int N = ROWS * LANES / PA_BLOCK;
+  static const int STEP = PA_BLOCK / LANES;     // rows of 256 lanes
   const __bf16* base;  // of the sequence's row 0
   long stride;
   int len, D;
+  unsigned from;       // of this thread's first load, bytes
+  bool has;            // whether its columns exist
 
+  __device__ PA_INLINE PaStage(const __bf16* base, long stride, int len,
+                               int D)
+      : base(base), stride(stride), len(len), D(D) {
+    const int r = threadIdx.x / LANES, in = threadIdx.x % LANES * (W / 2);
+    const int col = (((in >> 3) ^ pa_swz<DP>(r)) << 3) + (in & 7);
+    from = (unsigned)(r * (int)stride + col) * 2;
+    has = col < D;
+  }
   template <typename F>
   __device__ PA_INLINE void each(int row0, F f) {
     const int lane = threadIdx.x & 63;
@@ -245,12 +256,24 @@ struct PaStage {
     }
   }
   __device__ PA_INLINE void start(int row0, __bf16* tile) {
-    if constexpr (W > 2) {
-      const __bf16* at = base + (long)row0 * stride;
+    const __bf16* at = base + (long)row0 * stride;
+    if constexpr (STEP % 16 == 0) {
+      // the swizzle repeats: a thread's loads are rows apart
+      if (row0 + ROWS <= len) {
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        if (has) {
+#pragma unroll
+          for (int u = 0; u < N; ++u)
+            pa_to_lds<W>(at + u * STEP * stride, from,
+                         tile + (u * PA_BLOCK + wave * 64) * (W / 2));
+        }
+        return;
+      }
+    }
+    if constexpr (W > 2)
       each(row0, [&](int first, int, unsigned from) PA_INLINE {
         pa_to_lds<W>(at, from * 2, tile + first * (W / 2));
       });
-    }
   }
   __device__ PA_INLINE void arrive(int row0, __bf16* tile) {
     if constexpr (W > 2) {

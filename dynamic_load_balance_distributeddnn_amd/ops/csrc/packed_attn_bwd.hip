@@ -152,6 +152,16 @@ pa_bwd_q_kernel(const PaBwd p, const BiasArg bias) {
   const int row = w0 + col;
   const int len = it.len;
   const int whole = r0 / PA_STEP;  // tiles that all rows see whole
+  PaStage<DP, W> ks(pa_at(p.k, it.first, h / p.G), p.k.row, len, p.D);
+  PaStage<DP, W> vs(pa_at(p.v, it.first, h / p.G), p.v.row, len, p.D);
+  if (p.D < DP) {
+    pa_clear<DP>(s_k[0], 2 * PA_STEP);
+    pa_clear<DP>(s_v[0], 2 * PA_STEP);
+    __syncthreads();
+  }
+  // the first tile is under way before anything else is waited for
+  ks.start(it.begin * PA_STEP, s_k[it.begin & 1]);
+  vs.start(it.begin * PA_STEP, s_v[it.begin & 1]);
 
   float far_bias = 0.f;
   int far_from = 0;
@@ -217,8 +227,6 @@ pa_bwd_q_kernel(const PaBwd p, const BiasArg bias) {
 #pragma unroll
   for (int t = 0; t < DT; ++t) acc[t] = pa_zero16();
 
-  PaStage<DP, W> ks{pa_at(p.k, it.first, h / p.G), p.k.row, len, p.D};
-  PaStage<DP, W> vs{pa_at(p.v, it.first, h / p.G), p.v.row, len, p.D};
   float win = 0.f;
   auto start = [&](int k0, int buf) PA_INLINE {
     ks.start(k0, s_k[buf]);
@@ -269,11 +277,12 @@ pa_bwd_q_kernel(const PaBwd p, const BiasArg bias) {
       acc[d] = pa_mfma(frags.cols(x * 16 * DP * 2, d), w, acc[d]);
   };
 
-  // t < 0: the sweep's.
+  // t < 0: the sweep's; its tiles stay in their two buffers.
   auto any_tile = [&](int t) PA_INLINE {
-    const int k0 = (t < 0 ? t + it.end : t) * PA_STEP, buf = t & 1;
-    const int k1 = t == -1 ? 0 : k0 + PA_STEP;  // of the next tile
-    if (t + 1 < it.end) start(k1, buf ^ 1);
+    const int tile = t < 0 ? t + it.end : t;
+    const int k0 = tile * PA_STEP, buf = tile & 1;
+    const bool more = t + 1 < (sweep ? 0 : it.end);
+    if (more) start(k0 + PA_STEP, buf ^ 1);
     const bool works = k0 <= w0 + 31;
     bf16x8 w[4];
     frags = lanes.fresh(buf * TILE * 2);
@@ -303,7 +312,7 @@ pa_bwd_q_kernel(const PaBwd p, const BiasArg bias) {
         for (int x = 0; x < 4; ++x) product(w[x], x);
       }
     }
-    if (t + 1 < it.end) arrive(k1, buf ^ 1);
+    if (more) arrive(k0 + PA_STEP, buf ^ 1);
   };
   auto whole_tile = [&](int t) PA_INLINE {
     const int k0 = t * PA_STEP, buf = t & 1;
@@ -321,14 +330,9 @@ pa_bwd_q_kernel(const PaBwd p, const BiasArg bias) {
     if (more) arrive(k0 + PA_STEP, buf ^ 1);
   };
 
-  if (p.D < DP) {
-    pa_clear<DP>(s_k[0], 2 * PA_STEP);
-    pa_clear<DP>(s_v[0], 2 * PA_STEP);
-    __syncthreads();
-  }
   int t = sweep ? -it.end : it.begin;
-  start(it.begin * PA_STEP, t & 1);
-  arrive(it.begin * PA_STEP, t & 1);
+  if (BIAS && near(it.begin * PA_STEP)) win = window(it.begin * PA_STEP);
+  arrive(it.begin * PA_STEP, it.begin & 1);
   if (!sweep)  // then there are none
     for (; t < min(whole, it.end); ++t) whole_tile(t);
   for (; t < it.end; ++t) {
@@ -417,7 +421,7 @@ __device__ PA_INLINE void pa_bwd_kv_end(const PaBwd& p, void* out, long row,
 }
 
 template <int DP, int W, bool BIAS, typename BiasArg>
-__global__ void __launch_bounds__(PA_BLOCK, 2)
+__global__ void __launch_bounds__(PA_BLOCK, DP == 64 && !BIAS ? 3 : 2)
 pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
   const int KS = DP / 16, DT = DP / 32;
   const int ROWS = 32;  // of a streamed tile
@@ -453,6 +457,40 @@ pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
 
   float far_bias = 0.f, next_far = 0.f;  // of this and the next step
   int far_from = 0;
+  if constexpr (BIAS) far_from = bias.starts[bias.buckets - 1];
+
+  // The order of the steps: first the tiles that need neither a mask nor
+  // the table's sums, from the sequence's end backwards and every head of
+  // a tile in turn, so that the workgroups of a sequence read the same
+  // queries at the same time, from L2; then the others, head by head.
+  int other = min(PA_ROWS / ROWS, nt);  // tiles of the second part
+  if (BIAS && p.part)
+    other = min(max(other, (far_from + PA_ROWS + ROWS - 1) / ROWS), nt);
+  const int h0 = hk * p.G, bulk = (nt - other) * p.G;
+  // tile and head of a step
+  auto tile_of = [&](int s) PA_INLINE {
+    return s < bulk ? nt - 1 - s / p.G : other - 1 - (s - bulk) % other;
+  };
+  auto head_of = [&](int s) PA_INLINE {
+    return s < bulk ? s % p.G : (s - bulk) / other;
+  };
+  int step = it.begin, t = tile_of(step), g = head_of(step);
+
+  // all that the first step needs is under way before any is waited for
+  if (p.D < DP) {
+    pa_clear<DP>(s_q[0], 2 * ROWS);
+    pa_clear<DP>(s_g[0], 2 * ROWS);
+    pa_clear<DP>(s_v, PA_ROWS);
+    __syncthreads();
+  }
+  PaStage<DP, W, ROWS> qs(pa_at(p.q, it.first, h0 + g), p.q.row, len, p.D);
+  PaStage<DP, W, ROWS> gs(pa_at(p.go, it.first, h0 + g), p.go.row, len, p.D);
+  PaStage<DP, W, ROWS> vs(pa_at(p.v, it.first, hk), p.v.row, len, p.D);
+  for (int r = 0; r < PA_ROWS && c0 + r < len; r += ROWS)
+    vs.start(c0 + r, s_v + r * DP);
+  qs.start(c0 + t * ROWS, s_q[step & 1]);
+  gs.start(c0 + t * ROWS, s_g[step & 1]);
+
   if constexpr (BIAS) {
     for (int b = threadIdx.x; b < bias.buckets; b += PA_BLOCK)
       s_start[b] = bias.starts[b];
@@ -461,7 +499,6 @@ pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
     for (int x = threadIdx.x; x < min(p.G, PA_FARHEADS); x += PA_BLOCK)
       s_far[x] = pa_bias(pa_table(bias, bias.buckets - 1, p.H, hk * p.G + x),
                          bias.is_bf16);
-    far_from = bias.starts[bias.buckets - 1];
     __syncthreads();
     for (int n = threadIdx.x; n < PA_DISTANCES; n += PA_BLOCK)
       s_bucket[n] = pa_bucket(s_start, bias.buckets, n);
@@ -498,15 +535,10 @@ pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
 #pragma unroll
   for (int t = 0; t < DT; ++t) dk[t] = dv[t] = pa_zero16();
 
-  PaStage<DP, W, ROWS> qs{nullptr, p.q.row, len, p.D};
-  PaStage<DP, W, ROWS> gs{nullptr, p.go.row, len, p.D};
   unsigned win = 0;
   float st_l = 0.f, st_d = 0.f, st_m = 0.f;
-  auto start = [&](int q0, int h, int buf) PA_INLINE {
-    qs.base = pa_at(p.q, it.first, h);
-    gs.base = pa_at(p.go, it.first, h);
-    qs.start(q0, s_q[buf]);
-    gs.start(q0, s_g[buf]);
+  // what goes with a tile: its rows' statistics, its window
+  auto start_rows = [&](int q0, int h) PA_INLINE {
     if constexpr (BIAS) {
       const int g = h - hk * p.G;
       next_far = g < PA_FARHEADS
@@ -515,30 +547,32 @@ pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
                                bias.is_bf16);
       if (near(q0, next_far)) win = window(q0, h);
     }
-    if (threadIdx.x < ROWS) {
-      // rows behind the sequence: weights of exp2(-inf)
-      st_l = INFINITY;
-      st_d = st_m = 0.f;
-      const int r = q0 + (int)threadIdx.x;
-      if (r < len) {
-        const long at = (long)h * p.T + it.first + r;
-        if constexpr (BIAS) {
-          st_m = p.stats[2 * at];
-          st_l = p.stats[2 * at + 1];
-        } else {
-          st_l = p.stats[at];
-        }
-        st_d = p.delta[at];
-      }
+    const int r = min(q0 + (int)(threadIdx.x & (ROWS - 1)), len - 1);
+    const long at = (long)h * p.T + it.first + r;
+    if constexpr (BIAS) {
+      st_m = p.stats[2 * at];
+      st_l = p.stats[2 * at + 1];
+    } else {
+      st_l = p.stats[at];
     }
+    st_d = p.delta[at];
+  };
+  auto start = [&](int q0, int h, int buf) PA_INLINE {
+    qs.base = pa_at(p.q, it.first, h);
+    gs.base = pa_at(p.go, it.first, h);
+    qs.start(q0, s_q[buf]);
+    gs.start(q0, s_g[buf]);
+    start_rows(q0, h);
   };
   auto arrive = [&](int q0, int buf) PA_INLINE {
     qs.arrive(q0, s_q[buf]);
     gs.arrive(q0, s_g[buf]);
     const bool each = BIAS && near(q0, next_far);
+    // a tile of one bias: all in one
+    if (BIAS && !each) st_l -= next_far - st_m;
+    // rows behind the sequence: weights of exp2(-inf)
+    if (q0 + (int)threadIdx.x >= len) st_l = INFINITY;
     if (threadIdx.x < ROWS) {
-      // a tile of one bias: all in one
-      if (BIAS && !each) st_l -= next_far - st_m;
       s_l[buf][threadIdx.x] = st_l;
       s_delta[buf][threadIdx.x] = st_d;
       if (BIAS) s_m[buf][threadIdx.x] = st_m;
@@ -661,36 +695,9 @@ pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
     if (more) arrive(q1, buf ^ 1);
   };
 
-  if (p.D < DP) {
-    pa_clear<DP>(s_q[0], 2 * ROWS);
-    pa_clear<DP>(s_g[0], 2 * ROWS);
-    pa_clear<DP>(s_v, PA_ROWS);
-    __syncthreads();
-  }
-  {
-    PaStage<DP, W, ROWS> vs{pa_at(p.v, it.first, hk), p.v.row, len, p.D};
-    for (int r = 0; r < PA_ROWS && c0 + r < len; r += ROWS) {
-      vs.start(c0 + r, s_v + r * DP);
-      vs.arrive(c0 + r, s_v + r * DP);
-    }
-  }
-  // The order of the steps: first the tiles that need neither a mask nor
-  // the table's sums, from the sequence's end backwards and every head of
-  // a tile in turn, so that the workgroups of a sequence read the same
-  // queries at the same time, from L2; then the others, head by head.
-  int other = min(PA_ROWS / ROWS, nt);  // tiles of the second part
-  if (BIAS && p.part)
-    other = min(max(other, (far_from + PA_ROWS + ROWS - 1) / ROWS), nt);
-  const int h0 = hk * p.G, bulk = (nt - other) * p.G;
-  // tile and head of a step
-  auto tile_of = [&](int s) PA_INLINE {
-    return s < bulk ? nt - 1 - s / p.G : other - 1 - (s - bulk) % other;
-  };
-  auto head_of = [&](int s) PA_INLINE {
-    return s < bulk ? s % p.G : (s - bulk) / other;
-  };
-  int step = it.begin, t = tile_of(step), g = head_of(step);
-  start(c0 + t * ROWS, h0 + g, step & 1);
+  start_rows(c0 + t * ROWS, h0 + g);
+  for (int r = 0; r < PA_ROWS && c0 + r < len; r += ROWS)
+    vs.arrive(c0 + r, s_v + r * DP);
   arrive(c0 + t * ROWS, step & 1);
   auto go = [&](auto tile) PA_INLINE {
     const int q0 = c0 + t * ROWS;

@@ -67,6 +67,17 @@ pa_fwd_kernel(const PaFwd p, const BiasArg bias) {
   const int row = w0 + col;          // this lane's
   const int len = it.len;
   const int whole = r0 / PA_STEP;  // tiles that all rows see whole
+  PaStage<DP, W> ks(pa_at(p.k, it.first, h / p.G), p.k.row, len, p.D);
+  PaStage<DP, W> vs(pa_at(p.v, it.first, h / p.G), p.v.row, len, p.D);
+  if (p.D < DP) {
+    pa_clear<DP>(s_k[0], 2 * PA_STEP);
+    pa_clear<DP>(s_v[0], 2 * PA_STEP);
+    __syncthreads();
+  }
+  // the first tile is under way before anything else is waited for
+  ks.start(it.begin * PA_STEP, s_k[it.begin & 1]);
+  vs.start(it.begin * PA_STEP, s_v[it.begin & 1]);
+
   float far_bias = 0.f;
   int far_from = 0;
   if constexpr (BIAS) {
@@ -109,8 +120,6 @@ pa_fwd_kernel(const PaFwd p, const BiasArg bias) {
   const float mul = p.scale * PA_LOG2E;
   float a = mul, b = far_bias;
 
-  PaStage<DP, W> ks{pa_at(p.k, it.first, h / p.G), p.k.row, len, p.D};
-  PaStage<DP, W> vs{pa_at(p.v, it.first, h / p.G), p.v.row, len, p.D};
   float win = 0.f;
   auto start = [&](int k0, int buf) PA_INLINE {
     ks.start(k0, s_k[buf]);
@@ -123,12 +132,7 @@ pa_fwd_kernel(const PaFwd p, const BiasArg bias) {
     vs.arrive(k0, s_v[buf]);
     __syncthreads();
   };
-  if (p.D < DP) {
-    pa_clear<DP>(s_k[0], 2 * PA_STEP);
-    pa_clear<DP>(s_v[0], 2 * PA_STEP);
-    __syncthreads();
-  }
-  start(it.begin * PA_STEP, it.begin & 1);
+  if (BIAS && near(it.begin * PA_STEP)) win = window(it.begin * PA_STEP);
   arrive(it.begin * PA_STEP, it.begin & 1);
 
   const PaFrags<DP> lanes(s_tiles, lane);

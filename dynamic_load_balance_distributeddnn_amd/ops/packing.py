@@ -76,7 +76,7 @@ class PackedSequences:
         keys = -(-np.minimum((tile + 1) * TILE_ROWS, n) // 64)
         queries = -(-(n - tile * TILE_ROWS) // 32) * (heads // kv_heads)
         return (self._chunks(seq, tile, keys, heads, 8, 512),
-                self._chunks(seq, tile, queries, kv_heads, 16, 768))
+                self._chunks(seq, tile, queries, kv_heads, 12, 768))
 
     def _chunks(self, seq, tile, steps, heads, least, shares):
         # 512 workgroups run at a time, so the longest tile is what a launch
@@ -86,7 +86,9 @@ class PackedSequences:
         # 16 heads of 128, 90 -> 100 us where it is 1.3 times.  The key
         # tiles, longer and more uneven, want shorter chunks: one of 8192,
         # 32 heads of 128 over 8, backward uncut 2740 us, 512 shares 2260,
-        # 768 shares 2120, 1024 shares 2190.
+        # 768 shares 2120, 1024 shares 2190; but of no less than 12 steps:
+        # eight of 512, 16 heads of 128 over 4, backward with 8 at least
+        # 101 us, with 12 90, with 16 100, with 24 103.
         total = int(steps.sum()) * heads
         limit = max(least, total // shares)
         if len(steps) and int(steps.max()) <= 1.5 * total / 512:
