@@ -220,7 +220,8 @@ static RbArgs rb_args(int64_t H, int64_t Q, int64_t K, int64_t buckets,
                   ((int64_t)starts.size() == buckets ||
                    (int64_t)starts.size() * 2 == buckets),
               "position bias: 2 to 256 buckets");
-  TORCH_CHECK(H <= 65535 && Q < (1 << 22) && K < (1l << 31),
+  // 64 rows at least a workgroup where there are many
+  TORCH_CHECK(H <= 65535 && Q <= 65535 * 64 && K < (1l << 31),
               "position bias: sizes out of range");
   RbArgs a;
   a.H = H;
@@ -299,6 +300,25 @@ static variable_list once(variable_list grads, const char* name) {
   return (*error)(std::move(grads));
 }
 
+// A backward under capture hands its gradients to the nodes of its inputs.
+// One that an eager graph made on the default stream (the accumulator of a
+// leaf lives as long as a graph that reads the leaf) would draw that stream
+// into the capture, which ends the process: an error here instead.
+static void refuse_eager_inputs(const char* name) {
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() ==
+      c10::hip::CaptureStatus::None)
+    return;
+  const auto node = torch::autograd::get_current_node();
+  if (!node) return;
+  for (size_t i = 0; i < node->num_outputs(); ++i) {
+    if (!node->task_should_compute_output(i)) continue;
+    const auto stream = node->next_edge(i).function->stream();
+    TORCH_CHECK(!stream.has_value() || stream->id() != 0, name,
+                ": a backward pass is captured while an eager graph of the "
+                "same tensors is alive; drop that graph's results first");
+  }
+}
+
 static Tensor dense_last(const Tensor& t) {
   return t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous();
 }
@@ -327,6 +347,7 @@ struct PackedAttention
     return out[0];
   }
   static variable_list backward(AutogradContext* ctx, variable_list grad) {
+    refuse_eager_inputs("packed_causal_attention");
     const auto saved = ctx->get_saved_variables();
     auto& d = ctx->saved_data;
     const auto n = d["counts"].toIntVector();
@@ -366,6 +387,7 @@ struct PositionBias : public torch::autograd::Function<PositionBias> {
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grad) {
+    refuse_eager_inputs("relative_position_bias");
     variable_list out(5);
     {
       at::AutoGradMode off(false);

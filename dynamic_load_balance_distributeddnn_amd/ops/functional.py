@@ -15,6 +15,7 @@ coverage from it.
 from __future__ import annotations
 
 import math
+import operator
 
 import torch
 import torch.nn.functional as F
@@ -218,6 +219,7 @@ def relative_position_bias(table, q_len, k_len, max_distance=128,
                            torch.float64):
         raise TypeError(f"the bias table has to be floating, "
                         f"got {table.dtype}")
+    q_len, k_len = operator.index(q_len), operator.index(k_len)
     if q_len < 0 or k_len < 0:
         raise ValueError("lengths must not be negative")
     starts = checked_starts(table.shape[0], max_distance, bidirectional)
@@ -250,7 +252,8 @@ def packed_causal_attention(q, k, v, packing, scale=None, bias_table=None,
 
     ``bias_table`` [num_buckets, nhead] adds ``relative_position_bias`` of
     it to the scaled scores without forming the grid; entries of -inf take
-    their distances out, and a row left with nothing is zeros.  ``scale``
+    their distances out, and a row left with nothing is zeros (finite ones
+    beyond 1e37 count as 1e37 on the GPU).  ``scale``
     defaults to d ** -0.5.  What a masked position holds, an infinity or
     NaN even, does not reach a row that does not see it.
 
@@ -270,8 +273,9 @@ def packed_causal_attention(q, k, v, packing, scale=None, bias_table=None,
             and k.device == device == v.device):
         _refuse_packed_attention(q, k, v, packing)
     scale = qs[2] ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < math.inf:
-        raise ValueError(f"scale has to be positive and finite, got {scale}")
+    if not 1e-30 < scale < 1e30:  # and its like in fp32
+        raise ValueError("scale has to lie between 1e-30 and 1e30, "
+                         f"got {scale}")
     starts = ()
     if bias_table is not None:
         if bias_table.dim() != 2 or bias_table.shape[1] != qs[1]:

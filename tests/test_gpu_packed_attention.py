@@ -413,3 +413,94 @@ def test_autocast_casts_fp32():
         o = FD.packed_causal_attention(q.float(), k.float(), v.float(),
                                        packing)
     assert torch.equal(o, FD.packed_causal_attention(q, k, v, packing))
+
+
+def test_more_heads_share_a_key_than_their_biases_fit_in_lds():
+    lens = [9, 200]
+    q, k, v, do, table = _inputs(209, 40, 1, 64, buckets=32)
+    want, tol = attention(q, k, v, lens, do=do, table=table)
+    _check_all(_run(q, k, v, do, lens, table), want, tol)
+
+
+def test_offsets_past_32_bits():
+    """More than 2**31 elements.  The last sequences are held against the
+    definition: by themselves their key tiles are cut into other chunks,
+    whose sums round in another order."""
+    lens = [128] * 8198 + [77, 100]
+    rows = sum(lens)
+    assert rows * 16 * 128 > 2 ** 31
+    q, k, v, do, _ = _inputs(rows, 16, 4, 128)
+    got = _run(q, k, v, do, lens)
+    want, tol = attention(q[-177:], k[-177:], v[-177:], [77, 100],
+                          do=do[-177:])
+    _check_all({name: t[-177:] for name, t in got.items()}, want, tol)
+
+
+def test_head_stride_past_32_bits():
+    lens = [100, 33]
+    q, k, v, do, _ = _inputs(133, 2, 2, 64)
+    want = _run(q, k, v, do, lens)
+    far = torch.empty(2 ** 31 + 133 * 64, dtype=torch.bfloat16,
+                      device="cuda")
+    views = []
+    for t in (q, k, v):
+        view = far.as_strided((133, 2, 64), (64, 2 ** 31, 1))
+        view.copy_(t)
+        views.append(view)
+        got = _run(*(view if x is t else x for x in (q, k, v)), do, lens)
+        torch.cuda.synchronize()
+        for name in want:
+            assert torch.equal(got[name], want[name]), name
+
+
+def test_two_streams_at_once():
+    FD = _fd()
+    lens = [500, 700]
+    packing = FD.PackedSequences(lens, device="cuda")
+    sets = [_inputs(1200, 8, 2, 128, seed=s, buckets=32) for s in (0, 1)]
+    want = [_run(*x[:4], lens, x[4], packing=packing) for x in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [None, None]
+    for _ in range(3):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                x = sets[i]
+                got[i] = _run(*x[:4], lens, x[4], packing=packing)
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        for name in want[i]:
+            assert torch.equal(got[i][name], want[i][name]), (i, name)
+
+
+def test_backward_under_capture_beside_an_eager_graph_is_refused():
+    """The leaf's accumulator belongs to the eager graph's stream, which
+    must not be drawn into the capture; without that graph it works."""
+    FD = _fd()
+    lens = [40, 30]
+    q, k, v, do, table = _inputs(70, 2, 2, 64, buckets=32)
+    packing = FD.PackedSequences(lens, device="cuda")
+    want = _run(q, k, v, do, lens, table, packing=packing)
+    leaf = table.detach().requires_grad_()
+    eager = FD.packed_causal_attention(q, k, v, packing, bias_table=leaf)
+    grid = FD.relative_position_bias(leaf, 8, 8)
+    torch.cuda.synchronize()
+
+    def captured():
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            o = FD.packed_causal_attention(q, k, v, packing, bias_table=leaf)
+            out = torch.autograd.grad(o, leaf, do)[0]
+            b = FD.relative_position_bias(leaf, 8, 8)
+            return graph, out, torch.autograd.grad(b.sum(), leaf)[0]
+
+    with pytest.raises(RuntimeError, match="eager graph"):
+        captured()
+    del eager, grid
+    graph, out, _ = captured()
+    for _ in range(2):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want["dtable"])

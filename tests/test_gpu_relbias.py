@@ -156,6 +156,27 @@ def test_autocast_reads_the_master_in_bf16():
     _check_grad(grad, dout, which, 32, torch.float32)
 
 
+def test_offsets_past_32_bits():
+    FD = _fd()
+    heads, keys, tail = 2, 2 ** 30 + 5, 400
+    assert heads * keys > 2 ** 31
+    table = _table(32, heads, torch.bfloat16).requires_grad_()
+    out = FD.relative_position_bias(table, 1, keys)
+    far = table.detach()[31]
+    assert torch.equal(out[:, 0, -tail:],
+                       FD.relative_position_bias(table, 1, tail)[:, 0])
+    for start in (0, 2 ** 29, keys - tail - 1000):
+        assert bool((out[:, 0, start:start + 1000] == far[:, None]).all())
+    dout = torch.zeros_like(out)
+    dout[:, :, -tail:] = torch.randn(heads, 1, tail, device="cuda")
+    dout[:, :, :tail] = torch.randn(heads, 1, tail, device="cuda")
+    got, = torch.autograd.grad(out, table, dout)
+    ends = torch.cat([dout[:, :, :tail], dout[:, :, -tail:]], 2)
+    which = torch.cat([torch.full((1, tail), 31, device="cuda"),
+                       _buckets(1, tail, 32, 128, False)], 1)
+    _check_grad(got, ends, which, 32, torch.bfloat16)
+
+
 def test_empty():
     FD = _fd()
     table = _table(32, 4, torch.float32).requires_grad_()

@@ -165,7 +165,7 @@ def test_attention_refusals():
                 (q, k[:, :0], v[:, :0])):
         with pytest.raises(ValueError):
             call(*bad, pack)
-    for scale in (0.0, -1.0, math.inf, math.nan):
+    for scale in (0.0, -1.0, math.inf, math.nan, 1e-40, 1e40):
         with pytest.raises(ValueError):
             call(q, k, v, pack, scale=scale)
     for bad, far in ((table[:, :3], 128), (table[0], 128), (table, 4),
@@ -187,6 +187,8 @@ def test_bias_refusals():
             call(**args)
     with pytest.raises(TypeError):
         call(table.long(), 3, 3)
+    with pytest.raises(TypeError):
+        call(table, 3.5, 3)
     with pytest.raises(ValueError):
         layers.RelativePositionBias(2, num_buckets=1)
 
