@@ -22,13 +22,22 @@
 // with the number of keys that a row's average spreads over, so the first
 // 128 rows of a sequence, which can have few, take delta from a sweep over
 // their one or two key tiles beforehand.
+//
+// Measured, both kernels and their joins: one sequence of 8192, 32 heads of
+// 128 over 8, 1880 us (730 TFLOP/s by the formula's 5 products, 1020 by
+// the 7 performed); seven of 8192 in all, 16 heads over 4, 303 us; eight
+// of 512, 93 us; 20 of 35, 2 heads of 100, 26 us.  With a bias and its
+// gradient: five of 4096 in all, 16 heads of 64, 135 us.  Bound by the
+// matrix units where sequences are long, else by the longest workgroup:
+// the key kernel holds 128 keys for all heads of a group, so it is cut
+// finer than the others.
 #include "packed_attn.h"
 
 // ---- The table's gradient: sums of dS along its diagonals, then of the
 // diagonals of a bucket, all in a fixed order.  The last bucket is left
 // out: a row's dS sum to 0, so it is minus the sum of the others.
-#define PA_DISTANCES 512
-#define PA_FARHEADS 32
+#define PA_DISTANCES 512  // with that many sums a wave
+#define PA_FARHEADS 32    // of a group that LDS keeps the far bias of
 
 // Lane l gets the value of lane (l + N) & 31 of its half.
 template <int N>
@@ -131,6 +140,9 @@ __device__ PA_INLINE void pa_bwd_q_end(const PaBwd& p, long first, int row,
     }
 }
 
+// Three waves a SIMD where 168 registers do without spilling in the loop:
+// with a bias, heads of 64, 145 -> 142 us (five of 4096 in all); without
+// one 112 -> 117 us, so two there.  128 columns want 256 registers.
 template <int DP, int W, bool BIAS, typename BiasArg>
 __global__ void __launch_bounds__(PA_BLOCK, DP == 64 && BIAS ? 3 : 2)
 pa_bwd_q_kernel(const PaBwd p, const BiasArg bias) {
@@ -420,6 +432,10 @@ __device__ PA_INLINE void pa_bwd_kv_end(const PaBwd& p, void* out, long row,
     }
 }
 
+// Streamed tiles of 32 rows, for the two accumulators of 32 x DP a wave
+// that live through the loop.  Three waves a SIMD where 168 registers do:
+// with a bias they spill 14 values (135 -> 139 us the one way, 204 -> 200
+// the other), so two there.
 template <int DP, int W, bool BIAS, typename BiasArg>
 __global__ void __launch_bounds__(PA_BLOCK, DP == 64 && !BIAS ? 3 : 2)
 pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {

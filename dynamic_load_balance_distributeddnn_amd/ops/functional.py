@@ -327,6 +327,7 @@ def _refuse_packed_attention(q, k, v, packing):
 
 def _packed_attention_plain(q, k, v, packing, scale, bias_table,
                             max_distance):
+    packing.check_device(q.device)
     wide = torch.promote_types(q.dtype, torch.float32)
     group = q.shape[1] // k.shape[1]
     parts = []

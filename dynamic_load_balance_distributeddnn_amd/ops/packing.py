@@ -24,7 +24,8 @@ class PackedSequences:
     are host integers (zero is allowed), so they are checked here once and
     no kernel reads a length that nobody looked at.  Build one per batch
     and use it for all layers, forward and backward, on any stream; it has
-    to outlive a captured graph that used it.
+    to outlive a captured graph that used it.  With a ``device`` it is for
+    tensors of that device only.
 
     For each head layout it is used with it keeps two work lists on the
     device, of the query tiles and of the key tiles (``work``).
@@ -116,11 +117,19 @@ class PackedSequences:
         joins[:, 4] = parts[cut]
         return rows, len(which), int((parts * cut).sum())
 
+    def check_device(self, device):
+        own = self.device
+        if own is not None and (own.type != device.type or
+                                own.index not in (None, device.index)):
+            raise ValueError(f"the PackedSequences is for {own}, the "
+                             f"tensors are on {device}")
+
     def work(self, device, heads, kv_heads):
         """The work lists of one head layout on a device, made at its first
         use (not within a graph capture) and kept."""
         key = (device, heads, kv_heads)
         if key not in self._lists:
+            self.check_device(device)
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("use the PackedSequences once with these "
                                    "heads before the capture")

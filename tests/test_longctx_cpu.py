@@ -165,6 +165,8 @@ def test_attention_refusals():
                 (q, k[:, :0], v[:, :0])):
         with pytest.raises(ValueError):
             call(*bad, pack)
+    with pytest.raises(ValueError):
+        call(q, k, v, FD.PackedSequences([10], device="cuda"))
     for scale in (0.0, -1.0, math.inf, math.nan, 1e-40, 1e40):
         with pytest.raises(ValueError):
             call(q, k, v, pack, scale=scale)
