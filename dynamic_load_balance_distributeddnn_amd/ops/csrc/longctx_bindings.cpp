@@ -114,6 +114,7 @@ static PaWork pa_work(const Tensor& list, int64_t chunks, int64_t slots,
 static int64_t pa_tile(int64_t D) { return 128 * (D <= 64 ? 64 : 128); }
 
 typedef std::tuple<Tensor, int64_t, int64_t> WorkList;  // chunks, slots
+typedef c10::optional<WorkList> MaybeWork;
 
 // q [T, H, D], k and v [T, Hkv, D]; work: the packing's query tiles.  Rows
 // from `total` on belong to no sequence and come back as zeros.
@@ -328,7 +329,7 @@ struct PackedAttention
   static Tensor forward(AutogradContext* ctx, const Tensor& q0,
                         const Tensor& k0, const Tensor& v0,
                         const MaybeTensor& table0, WorkList work_q,
-                        WorkList work_kv, int64_t total, double scale,
+                        MaybeWork work_kv, int64_t total, double scale,
                         std::vector<int64_t> starts, bool table_grad) {
     const Tensor q = dense_last(q0), k = dense_last(k0), v = dense_last(v0);
     MaybeTensor table;
@@ -336,11 +337,13 @@ struct PackedAttention
     auto out = packed_attn_fwd(q, k, v, work_q, total, scale, table, starts);
     ctx->save_for_backward({q, k, v, out[0], out[1],
                             table.has_value() ? *table : Tensor(),
-                            std::get<0>(work_q), std::get<0>(work_kv)});
+                            std::get<0>(work_q),
+                            work_kv ? std::get<0>(*work_kv) : Tensor()});
     auto& d = ctx->saved_data;
     d["counts"] = std::vector<int64_t>{
-        std::get<1>(work_q), std::get<2>(work_q), std::get<1>(work_kv),
-        std::get<2>(work_kv), total};
+        std::get<1>(work_q), std::get<2>(work_q),
+        work_kv ? std::get<1>(*work_kv) : 0,
+        work_kv ? std::get<2>(*work_kv) : 0, total};
     d["scale"] = scale;
     d["starts"] = std::move(starts);
     d["table_grad"] = table_grad;
@@ -370,7 +373,7 @@ struct PackedAttention
 
 static Tensor packed_attention(Tensor q, Tensor k, Tensor v,
                                MaybeTensor table, WorkList work_q,
-                               WorkList work_kv, int64_t total, double scale,
+                               MaybeWork work_kv, int64_t total, double scale,
                                std::vector<int64_t> starts) {
   return PackedAttention::apply(
       q, k, v, table, work_q, work_kv, total, scale, starts,

@@ -27,8 +27,8 @@ class PackedSequences:
     to outlive a captured graph that used it.  With a ``device`` it is for
     tensors of that device only.
 
-    For each head layout it is used with it keeps two work lists on the
-    device, of the query tiles and of the key tiles (``work``).
+    For each head layout it is used with it keeps work lists on the device,
+    of the query tiles and, for gradients, of the key tiles.
     """
 
     def __init__(self, lengths, device=None):
@@ -63,38 +63,74 @@ class PackedSequences:
         seq = np.repeat(np.arange(len(tiles)), tiles)
         return seq, np.arange(len(seq)) - (np.cumsum(tiles) - tiles)[seq]
 
-    def host_work(self, heads, kv_heads):
-        """((list, chunks, slots) of the query tiles, of the key tiles).
+    def host_work(self, heads, kv_heads, at_once=512):
+        """((list, chunks, slots) of the query tiles, of the key tiles)."""
+        return (self._query_work(heads),
+                self._key_work(heads, kv_heads, at_once))
 
-        A query tile reads the 64-key tiles up to its last row; a key tile
-        is read by the 32-row tiles from its first row on, of every head
-        that shares it.  Tiles with much more to do than a workgroup's
-        share of the whole are cut into chunks, whose sums a second kernel
-        joins; the chunks come with the longest first.
-        """
+    def _query_work(self, heads):
+        """A query tile reads the 64-key tiles up to its last row.  Tiles
+        with much more to do than a workgroup's share of the whole are cut
+        into chunks, whose sums a second kernel joins."""
         seq, tile = self._tiles()
-        n = self._n[seq]
-        keys = -(-np.minimum((tile + 1) * TILE_ROWS, n) // 64)
-        queries = -(-(n - tile * TILE_ROWS) // 32) * (heads // kv_heads)
-        return (self._chunks(seq, tile, keys, heads, 8, 512),
-                self._chunks(seq, tile, queries, kv_heads, 12, 768))
-
-    def _chunks(self, seq, tile, steps, heads, least, shares):
+        steps = -(-np.minimum((tile + 1) * TILE_ROWS, self._n[seq]) // 64)
+        total = int(steps.sum()) * heads
         # 512 workgroups run at a time, so the longest tile is what a launch
         # takes at least.  Cutting costs a trip of the sums through memory:
         # one sequence of 4001, 12 heads of 64, forward 85 -> 63 us where
         # the longest is 2.7 times a place's share, but 7 packed ones,
-        # 16 heads of 128, 90 -> 100 us where it is 1.3 times.  The key
-        # tiles, longer and more uneven, want shorter chunks: one of 8192,
-        # 32 heads of 128 over 8, backward uncut 2740 us, 512 shares 2260,
-        # 768 shares 2120, 1024 shares 2190; but of no less than 12 steps:
-        # eight of 512, 16 heads of 128 over 4, backward with 8 at least
-        # 101 us, with 12 90, with 16 100, with 24 103.
-        total = int(steps.sum()) * heads
-        limit = max(least, total // shares)
+        # 16 heads of 128, 90 -> 100 us where it is 1.3 times.
+        limit = max(8, total // 512)
         if len(steps) and int(steps.max()) <= 1.5 * total / 512:
             limit = int(steps.max())
+        return self._chunks(seq, tile, steps, limit)
+
+    def _key_work(self, heads, kv_heads, at_once):
+        """A key tile is read by the 32-row tiles from its first row on, of
+        every head that shares it; ``at_once`` workgroups run at a time.
+
+        These are longer and more uneven, and how well the chunks of a
+        limit fill the places decides: the limit is the best of a few by
+        what their launch and join take, in steps.  A chunk costs 8 of its
+        own, a join 2.5 and 0.012 each chunk and head (measured, 1.2 to 2
+        us a step).  Backward in us, with limits of a share of the whole by
+        384, 512, 640 and 768, the one taken last: one of 8192, 16 heads of
+        64 over 4, 661, 589, 565, 654 (640); five of 4096 in all, 16 heads
+        of 64 with a bias, 124, 132, 134, 134 (384); one of 8192, 32 heads
+        of 128 over 8, 2109, 2040, 1968, 1912 (768).  Below 12 steps chunks
+        lose: eight of 512, 16 heads of 128 over 4, 106 us with 8, 91 with
+        12, 100 with 16.
+        """
+        seq, tile = self._tiles()
+        steps = (-(-(self._n[seq] - tile * TILE_ROWS) // 32)
+                 * (heads // kv_heads))
+        longest = int(steps.max()) if len(steps) else 0
+        total = int(steps.sum()) * kv_heads
+        # many tiles a place: nothing to gain by cutting
+        if 2 * longest * at_once <= total or longest <= 12:
+            return self._chunks(seq, tile, steps, longest)
+        limits = {max(12, total // n) for n in (384, 512, 640, 768)}
+        limit = min(sorted(limits | {longest}),
+                    key=lambda x: self._time(steps, kv_heads, x, at_once))
+        return self._chunks(seq, tile, steps, limit)
+
+    @staticmethod
+    def _time(steps, heads, limit, at_once):
         parts = -(-steps // limit)
+        sizes = np.sort(np.repeat(steps / parts, parts * heads))[::-1] + 8
+        # the longest first, each to the place that is free first
+        load = np.zeros(at_once)
+        for i in range(0, len(sizes), at_once):
+            part = sizes[i:i + at_once]
+            load[:len(part)] += part
+            load.sort()
+        slots = int((parts * (parts > 1)).sum()) * heads
+        return load[-1] + (2.5 + 0.012 * slots if slots else 0.0)
+
+    def _chunks(self, seq, tile, steps, limit):
+        """Chunks of at most ``limit`` steps, the longest first, then the
+        joins of the tiles that are in several."""
+        parts = -(-steps // max(limit, 1))
         which = np.repeat(np.arange(len(steps)), parts)
         part = np.arange(len(which)) - (np.cumsum(parts) - parts)[which]
         cut = parts > 1
@@ -124,23 +160,30 @@ class PackedSequences:
             raise ValueError(f"the PackedSequences is for {own}, the "
                              f"tensors are on {device}")
 
-    def work(self, device, heads, kv_heads):
-        """The work lists of one head layout on a device, made at its first
-        use (not within a graph capture) and kept."""
-        key = (device, heads, kv_heads)
+    def query_work(self, device, heads):
+        """The query tiles' work list on a device, made at its first use
+        (not within a graph capture) and kept."""
+        key = (device, heads)
         if key not in self._lists:
-            self.check_device(device)
-            if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("use the PackedSequences once with these "
-                                   "heads before the capture")
-            lists = self.host_work(heads, kv_heads)
-            both = np.concatenate([rows for rows, _, _ in lists])
-            # a synchronous copy: the lists are there for every stream
-            both = torch.from_numpy(both).to(device)
-            cut = len(lists[0][0])
-            self._lists[key] = ((both[:cut], *lists[0][1:]),
-                                (both[cut:], *lists[1][1:]))
+            self._lists[key] = self._put(device, self._query_work, heads)
         return self._lists[key]
+
+    def key_work(self, device, heads, kv_heads, at_once):
+        """The key tiles', as ``query_work``; only a backward reads it."""
+        key = (device, heads, kv_heads, at_once)
+        if key not in self._lists:
+            self._lists[key] = self._put(device, self._key_work, heads,
+                                         kv_heads, at_once)
+        return self._lists[key]
+
+    def _put(self, device, make, *args):
+        self.check_device(device)
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("use the PackedSequences once in this way "
+                               "before the capture")
+        rows, chunks, slots = make(*args)
+        # a synchronous copy: the list is there for every stream
+        return torch.from_numpy(rows).to(device), chunks, slots
 
 
 @lru_cache(maxsize=64)
