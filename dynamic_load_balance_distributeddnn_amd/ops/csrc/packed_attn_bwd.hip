@@ -811,33 +811,47 @@ pa_bwd_kv_join_kernel(const PaBwd p) {
                         blockIdx.y >> 1, v ? 1.f : p.scale);
 }
 
-// dtable[b, h] from the chunks' partial sums; a workgroup a head, a wave a
-// bucket at a time, every sum in a fixed order.
-__global__ void __launch_bounds__(PA_BLOCK)
+// dtable[b, h] from the chunks' partial sums; a workgroup a head, a lane a
+// bucket, the chunks by turns to the waves, every sum in a fixed order.  42
+// chunks of 16 heads: 2 us less than a wave a bucket and a lane a chunk.
+#define PA_TABLE_WAVES 16
+__global__ void __launch_bounds__(PA_TABLE_WAVES * 64)
 pa_table_grad_kernel(const float* __restrict__ part, void* out, int is_bf16,
                      long chunks, int H, int buckets) {
+  __shared__ float s_part[PA_TABLE_WAVES][64];
   __shared__ float s_sum[PA_MAXBUCKETS];
-  const int h = blockIdx.x, lane = threadIdx.x & 63;
-  for (int b = threadIdx.x >> 6; b < buckets - 1; b += PA_BLOCK / 64) {
-    float v = 0.f;
-    for (long i = lane; i < chunks; i += 64)
-      v += part[(i * H + h) * buckets + b];
-    v = wave_reduce_sum(v);
-    if (lane == 0) s_sum[b] = v;
+  const int h = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int b0 = 0; b0 < buckets; b0 += 64) {
+    const int b = min(b0 + lane, buckets - 1);
+    float v[4] = {};
+    for (long i = wave; i < chunks; i += 4 * PA_TABLE_WAVES)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const long at = i + u * PA_TABLE_WAVES;
+        const float x = part[(min(at, chunks - 1) * H + h) * buckets + b];
+        v[u] += at < chunks ? x : 0.f;
+      }
+    s_part[wave][lane] = (v[0] + v[1]) + (v[2] + v[3]);
+    __syncthreads();
+    if (wave == 0) {
+      float x = 0.f;
+#pragma unroll
+      for (int w = 0; w < PA_TABLE_WAVES; ++w) x += s_part[w][lane];
+      if (b0 + lane < buckets) s_sum[b0 + lane] = x;
+    }
+    __syncthreads();
   }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    float all = 0.f;
-    for (int b = 0; b < buckets - 1; ++b) all += s_sum[b];
-    s_sum[buckets - 1] = -all;
-  }
-  __syncthreads();
-  for (int b = threadIdx.x; b < buckets; b += PA_BLOCK) {
+  if (wave > 0) return;
+  float all = 0.f;
+  for (int b = lane; b < buckets - 1; b += 64) all += s_sum[b];
+  all = __shfl(wave_reduce_sum(all), 0, 64);
+  for (int b = lane; b < buckets; b += 64) {
+    const float x = b < buckets - 1 ? s_sum[b] : -all;
     const long at = (long)b * H + h;
     if (is_bf16)
-      static_cast<__bf16*>(out)[at] = (__bf16)s_sum[b];
+      static_cast<__bf16*>(out)[at] = (__bf16)x;
     else
-      static_cast<float*>(out)[at] = s_sum[b];
+      static_cast<float*>(out)[at] = x;
   }
 }
 
@@ -881,7 +895,7 @@ extern "C" void dlb_packed_attn_bwd(const PaBwd* p, const PaBias* bias,
   else if (width == 4) go(pa_bwd_go<64, 4>, pa_bwd_go<128, 4>);
   else go(pa_bwd_go<64, 2>, pa_bwd_go<128, 2>);
   if (bias && dtable)
-    hipLaunchKernelGGL(pa_table_grad_kernel, dim3(p->H), dim3(PA_BLOCK), 0,
-                       stream, p->part, dtable, dtable_bf16,
-                       (long)p->work_kv.n_chunks, p->H, bias->buckets);
+    hipLaunchKernelGGL(pa_table_grad_kernel, dim3(p->H),
+                       dim3(PA_TABLE_WAVES * 64), 0, stream, p->part, dtable,
+                       dtable_bf16, (long)p->work_kv.n_chunks, p->H, bias->buckets);
 }
