@@ -432,15 +432,22 @@ __device__ PA_INLINE void pa_bwd_kv_end(const PaBwd& p, void* out, long row,
     }
 }
 
-// Streamed tiles of 32 rows, for the two accumulators of 32 x DP a wave
-// that live through the loop.  Three waves a SIMD where 168 registers do:
+// Rows of a streamed tile: the two accumulators of 32 x DP a wave live
+// through the loop, and LDS holds two tiles of queries and two of gradients
+// next to 128 values, for two workgroups a CU.
+template <int DP>
+struct PaKeys {
+  static const int ROWS = DP == 64 ? 64 : 32;
+};
+
+//  Three waves a SIMD where 168 registers do:
 // with a bias they spill 14 values (135 -> 139 us the one way, 204 -> 200
 // the other), so two there.
 template <int DP, int W, bool BIAS, typename BiasArg>
 __global__ void __launch_bounds__(PA_BLOCK, DP == 64 && !BIAS ? 3 : 2)
 pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
   const int KS = DP / 16, DT = DP / 32;
-  const int ROWS = 32;  // of a streamed tile
+  const int ROWS = PaKeys<DP>::ROWS;  // of a streamed tile
   const int TILE = ROWS * DP;
   __shared__ __attribute__((aligned(1024)))
   __bf16 s_tiles[4 + PA_ROWS / ROWS][TILE];
@@ -603,17 +610,18 @@ pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
 
   const PaFrags<DP> lanes(s_tiles, lane);
   PaFrags<DP> frags = lanes;  // of the current buffer
-  // s: the weights, dp: their gradient, of 32 queries of a tile
-  auto gradient = [&](f32x16& s, f32x16& dp, int q0,
+  // s: the weights, dp: their gradient, of queries 32 j .. of a tile
+  auto gradient = [&](f32x16& s, f32x16& dp, int q0, int j,
                       int buf) PA_INLINE {
+    const unsigned from = j * 32 * DP * 2;
     const PaFrags<DP> vfrags = lanes.fresh(wave * (32 * DP * 2));
     s = dp = pa_zero16();
 #pragma unroll
     for (int x = 0; x < KS; ++x)
-      s = pa_mfma(frags.rows(0, x), kf[x], s);
+      s = pa_mfma(frags.rows(from, x), kf[x], s);
 #pragma unroll
     for (int x = 0; x < KS; ++x)
-      dp = pa_mfma(frags.rows(2 * TILE * 2, x),
+      dp = pa_mfma(frags.rows(from + 2 * TILE * 2, x),
                    vfrags.rows(4 * TILE * 2, x), dp);
     bool each = false;
     if constexpr (BIAS) each = near(q0, far_bias);
@@ -622,7 +630,7 @@ pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
       const float* w = s_win[BIAS ? buf : 0] + PA_ROWS - 1 - wave * 32 - col;
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const int at = 8 * g + 4 * half;
+        const int at = 32 * j + 8 * g + 4 * half;
         const f32x4 mv = *reinterpret_cast<const f32x4*>(
             &s_m[buf][BIAS ? at : 0]);
 #pragma unroll
@@ -632,7 +640,7 @@ pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
     }
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      const int at = 8 * g + 4 * half;
+      const int at = 32 * j + 8 * g + 4 * half;
       const f32x4 lv = *reinterpret_cast<const f32x4*>(&s_l[buf][at]);
       const f32x4 ev = *reinterpret_cast<const f32x4*>(&s_delta[buf][at]);
 #pragma unroll
@@ -657,6 +665,7 @@ pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
       }
     }
   };
+  // with 16 of its queries, 16 x ..
   auto product = [&](bf16x8 pw, bf16x8 sw, int x) PA_INLINE {
 #pragma unroll
     for (int d = 0; d < DT; ++d)
@@ -672,16 +681,23 @@ pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
     const int buf = step & 1;
     const bool more = step + 1 < it.end;
     if (more) start(q1, h1, buf ^ 1);
-    const bool works = q0 + ROWS - 1 >= w0;
     frags = lanes.fresh(buf * TILE * 2);
-    f32x16 s, dp;
-    if (works) {
-      gradient(s, dp, q0, buf);
-      const int lim = key - q0 - 4 * half;
+    bf16x8 pw[ROWS / 16], sw[ROWS / 16];
+#pragma unroll
+    for (int j = 0; j < ROWS / 32; ++j) {
+      if (q0 + 32 * j + 31 < w0) continue;
+      f32x16 s, dp;
+      gradient(s, dp, q0, j, buf);
+      const int lim = key - q0 - 32 * j - 4 * half;
 #pragma unroll
       for (int r = 0; r < 16; ++r)
         if (8 * (r >> 2) + (r & 3) < lim) s[r] = dp[r] = 0.f;
-      table_sums(dp, q0);
+      table_sums(dp, q0 + 32 * j);
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        pw[2 * j + x] = pa_operand(s, x);
+        sw[2 * j + x] = pa_operand(dp, x);
+      }
     }
     if (__syncthreads_or(pa_tile_nonfinite<DP, ROWS>(s_q[buf]) ||
                          pa_tile_nonfinite<DP, ROWS>(s_g[buf]))) {
@@ -692,10 +708,9 @@ pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
       pa_cleanse<DP, ROWS>(s_q[buf]);
       __syncthreads();
     }
-    if (works) {
-      product(pa_operand(s, 0), pa_operand(dp, 0), 0);
-      product(pa_operand(s, 1), pa_operand(dp, 1), 1);
-    }
+#pragma unroll
+    for (int x = 0; x < ROWS / 16; ++x)
+      if (q0 + 32 * (x >> 1) + 31 >= w0) product(pw[x], sw[x], x);
     if (more) arrive(q1, buf ^ 1);
   };
   auto whole_tile = [&](int step, int q0, int q1, int h1) PA_INLINE {
@@ -703,11 +718,14 @@ pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
     const bool more = step + 1 < it.end;
     if (more) start(q1, h1, buf ^ 1);
     frags = lanes.fresh(buf * TILE * 2);
-    f32x16 s, dp;
-    gradient(s, dp, q0, buf);
-    table_sums(dp, q0);
-    product(pa_operand(s, 0), pa_operand(dp, 0), 0);
-    product(pa_operand(s, 1), pa_operand(dp, 1), 1);
+#pragma unroll
+    for (int j = 0; j < ROWS / 32; ++j) {
+      f32x16 s, dp;
+      gradient(s, dp, q0, j, buf);
+      table_sums(dp, q0 + 32 * j);
+      product(pa_operand(s, 0), pa_operand(dp, 0), 2 * j);
+      product(pa_operand(s, 1), pa_operand(dp, 1), 2 * j + 1);
+    }
     if (more) arrive(q1, buf ^ 1);
   };
 

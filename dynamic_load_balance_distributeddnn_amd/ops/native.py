@@ -279,9 +279,11 @@ def packed_causal_attention(q, k, v, packing, scale, table, starts):
     if torch.is_grad_enabled() and (
             q.requires_grad or k.requires_grad or v.requires_grad
             or table is not None and table.requires_grad):
-        # what the key kernel's registers let run at a time
-        at_once = 768 if q.shape[2] <= 64 and table is None else 512
-        work_kv = packing.key_work(q.device, heads, k.shape[1], at_once)
+        # the key kernel's tiles, and what its registers let run at a time
+        small = q.shape[2] <= 64
+        work_kv = packing.key_work(q.device, heads, k.shape[1],
+                                   64 if small else 32,
+                                   768 if small and table is None else 512)
     work_q = packing.query_work(q.device, heads)
     return ext().packed_attention(q, k, v, table, work_q, work_kv,
                                   packing.total, scale, starts)

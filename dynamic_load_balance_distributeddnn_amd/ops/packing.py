@@ -63,10 +63,10 @@ class PackedSequences:
         seq = np.repeat(np.arange(len(tiles)), tiles)
         return seq, np.arange(len(seq)) - (np.cumsum(tiles) - tiles)[seq]
 
-    def host_work(self, heads, kv_heads, at_once=512):
+    def host_work(self, heads, kv_heads, rows=32, at_once=512):
         """((list, chunks, slots) of the query tiles, of the key tiles)."""
         return (self._query_work(heads),
-                self._key_work(heads, kv_heads, at_once))
+                self._key_work(heads, kv_heads, rows, at_once))
 
     def _query_work(self, heads):
         """A query tile reads the 64-key tiles up to its last row.  Tiles
@@ -85,15 +85,16 @@ class PackedSequences:
             limit = int(steps.max())
         return self._chunks(seq, tile, steps, limit)
 
-    def _key_work(self, heads, kv_heads, at_once):
-        """A key tile is read by the 32-row tiles from its first row on, of
-        every head that shares it; ``at_once`` workgroups run at a time.
+    def _key_work(self, heads, kv_heads, rows, at_once):
+        """A key tile is read by the tiles of ``rows`` queries from its
+        first row on, of every head that shares it; ``at_once`` workgroups
+        run at a time.
 
         These are longer and more uneven, and how well the chunks of a
         limit fill the places decides: the limit is the best of a few by
         what their launch and join take, in steps.  A chunk costs 8 of its
         own, a join 2.5 and 0.012 each chunk and head (measured, 1.2 to 2
-        us a step).  Backward in us, with limits of a share of the whole by
+        us a step; all for steps of 32 rows).  Backward in us, with limits of a share of the whole by
         384, 512, 640 and 768, the one taken last: one of 8192, 16 heads of
         64 over 4, 661, 589, 565, 654 (640); five of 4096 in all, 16 heads
         of 64 with a bias, 124, 132, 134, 134 (384); one of 8192, 32 heads
@@ -102,22 +103,25 @@ class PackedSequences:
         12, 100 with 16.
         """
         seq, tile = self._tiles()
-        steps = (-(-(self._n[seq] - tile * TILE_ROWS) // 32)
+        steps = (-(-(self._n[seq] - tile * TILE_ROWS) // rows)
                  * (heads // kv_heads))
         longest = int(steps.max()) if len(steps) else 0
         total = int(steps.sum()) * kv_heads
+        least = 12 * 32 // rows
         # many tiles a place: nothing to gain by cutting
-        if 2 * longest * at_once <= total or longest <= 12:
+        if 2 * longest * at_once <= total or longest <= least:
             return self._chunks(seq, tile, steps, longest)
-        limits = {max(12, total // n) for n in (384, 512, 640, 768)}
+        limits = {max(least, total // n) for n in (384, 512, 640, 768)}
         limit = min(sorted(limits | {longest}),
-                    key=lambda x: self._time(steps, kv_heads, x, at_once))
+                    key=lambda x: self._time(steps, kv_heads, x, at_once,
+                                             32 / rows))
         return self._chunks(seq, tile, steps, limit)
 
     @staticmethod
-    def _time(steps, heads, limit, at_once):
+    def _time(steps, heads, limit, at_once, unit):
         parts = -(-steps // limit)
-        sizes = np.sort(np.repeat(steps / parts, parts * heads))[::-1] + 8
+        sizes = np.sort(np.repeat(steps / parts, parts * heads))[::-1]
+        sizes = sizes + 8 * unit
         # the longest first, each to the place that is free first
         load = np.zeros(at_once)
         for i in range(0, len(sizes), at_once):
@@ -125,7 +129,7 @@ class PackedSequences:
             load[:len(part)] += part
             load.sort()
         slots = int((parts * (parts > 1)).sum()) * heads
-        return load[-1] + (2.5 + 0.012 * slots if slots else 0.0)
+        return load[-1] + ((2.5 + 0.012 * slots) * unit if slots else 0.0)
 
     def _chunks(self, seq, tile, steps, limit):
         """Chunks of at most ``limit`` steps, the longest first, then the
@@ -168,12 +172,12 @@ class PackedSequences:
             self._lists[key] = self._put(device, self._query_work, heads)
         return self._lists[key]
 
-    def key_work(self, device, heads, kv_heads, at_once):
+    def key_work(self, device, heads, kv_heads, rows, at_once):
         """The key tiles', as ``query_work``; only a backward reads it."""
-        key = (device, heads, kv_heads, at_once)
+        key = (device, heads, kv_heads, rows, at_once)
         if key not in self._lists:
             self._lists[key] = self._put(device, self._key_work, heads,
-                                         kv_heads, at_once)
+                                         kv_heads, rows, at_once)
         return self._lists[key]
 
     def _put(self, device, make, *args):
