@@ -25,9 +25,10 @@
 //
 // Measured, both kernels and their joins: one sequence of 8192, 32 heads of
 // 128 over 8, 1880 us (730 TFLOP/s by the formula's 5 products, 1020 by
-// the 7 performed); seven of 8192 in all, 16 heads over 4, 303 us; eight
-// of 512, 93 us; 20 of 35, 2 heads of 100, 26 us.  With a bias and its
-// gradient: five of 4096 in all, 16 heads of 64, 135 us.  Bound by the
+// the 7 performed); seven of 8192 in all, 16 heads over 4, 290 us; eight
+// of 512, 92 us; 20 of 35, 2 heads of 100, 26 us.  With a bias and its
+// gradient: five of 4096 in all, 16 heads of 64, 111 us; one of 4001, 12
+// heads, 173.  Bound by the
 // matrix units where sequences are long, else by the longest workgroup:
 // the key kernel holds 128 keys for all heads of a group, so it is cut
 // finer than the others.
@@ -432,17 +433,16 @@ __device__ PA_INLINE void pa_bwd_kv_end(const PaBwd& p, void* out, long row,
     }
 }
 
-// Rows of a streamed tile: the two accumulators of 32 x DP a wave live
-// through the loop, and LDS holds two tiles of queries and two of gradients
-// next to 128 values, for two workgroups a CU.
+// Rows of a streamed tile: LDS holds two tiles of queries and two of
+// gradients next to 128 values, for two workgroups a CU.  Heads of 64 with
+// 32 rows: 198 us for 177 (one of 4001, 12 heads, a bias).
 template <int DP>
 struct PaKeys {
   static const int ROWS = DP == 64 ? 64 : 32;
 };
 
-//  Three waves a SIMD where 168 registers do:
-// with a bias they spill 14 values (135 -> 139 us the one way, 204 -> 200
-// the other), so two there.
+// Three waves a SIMD where 168 registers do; with a bias they spill (five
+// of 4096 in all, 16 heads of 64: 119 -> 159 us), so two there.
 template <int DP, int W, bool BIAS, typename BiasArg>
 __global__ void __launch_bounds__(PA_BLOCK, DP == 64 && !BIAS ? 3 : 2)
 pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {

@@ -77,11 +77,14 @@ class PackedSequences:
         total = int(steps.sum()) * heads
         # 512 workgroups run at a time, so the longest tile is what a launch
         # takes at least.  Cutting costs a trip of the sums through memory:
-        # one sequence of 4001, 12 heads of 64, forward 85 -> 63 us where
-        # the longest is 2.7 times a place's share, but 7 packed ones,
-        # 16 heads of 128, 90 -> 100 us where it is 1.3 times.
-        limit = max(8, total // 512)
-        if len(steps) and int(steps.max()) <= 1.5 * total / 512:
+        # one sequence of 4001, 12 heads of 64, forward 73 -> 50 us where
+        # the longest is 2.7 times a place's share, but seven packed ones,
+        # 16 heads of 128 over 4, 79 -> 85 where it is 1.3 times, and six of
+        # 1024, 12 heads of 64, 26 -> 30 where it is 1.6 times.  Chunks of
+        # a 384th, the unequal ones then fill the places: five of 4096 in
+        # all, 16 heads of 128, 46 us, with a 512th 50, a 768th 53.
+        limit = max(8, total // 384)
+        if len(steps) and int(steps.max()) <= 1.75 * total / 512:
             limit = int(steps.max())
         return self._chunks(seq, tile, steps, limit)
 
@@ -96,11 +99,11 @@ class PackedSequences:
         own, a join 2.5 and 0.012 each chunk and head (measured, 1.2 to 2
         us a step; all for steps of 32 rows).  Backward in us, with limits of a share of the whole by
         384, 512, 640 and 768, the one taken last: one of 8192, 16 heads of
-        64 over 4, 661, 589, 565, 654 (640); five of 4096 in all, 16 heads
-        of 64 with a bias, 124, 132, 134, 134 (384); one of 8192, 32 heads
+        64 over 4, 621, 572, 560, 623 (640); five of 4096 in all, 16 heads
+        of 64 with a bias, 114, 118, 126, 125 (384); one of 8192, 32 heads
         of 128 over 8, 2109, 2040, 1968, 1912 (768).  Below 12 steps chunks
-        lose: eight of 512, 16 heads of 128 over 4, 106 us with 8, 91 with
-        12, 100 with 16.
+        lose: eight of 512, 16 heads of 128 over 4, 102 us with 8, 91 with
+        12, 98 with 16.
         """
         seq, tile = self._tiles()
         steps = (-(-(self._n[seq] - tile * TILE_ROWS) // rows)
