@@ -504,3 +504,14 @@ def test_backward_under_capture_beside_an_eager_graph_is_refused():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want["dtable"])
+
+
+@pytest.mark.parametrize("heads,kv,d", [(4, 2, 64), (2, 2, 128), (6, 1, 40)])
+@pytest.mark.parametrize("buckets,far", [(32, 128), (64, 2000)])
+def test_bias_over_tiles_in_several_chunks(heads, kv, d, buckets, far):
+    """Long sequences on few heads: every list is cut, the table's sums
+    come by distance or, beyond 512 of them, by bucket."""
+    lens = [2500, 900, 33]
+    q, k, v, do, table = _inputs(sum(lens), heads, kv, d, buckets=buckets)
+    want, tol = attention(q, k, v, lens, table=table, far=far, do=do)
+    _check_all(_run(q, k, v, do, lens, table, far), want, tol)
