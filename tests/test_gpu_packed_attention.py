@@ -515,3 +515,15 @@ def test_bias_over_tiles_in_several_chunks(heads, kv, d, buckets, far):
     q, k, v, do, table = _inputs(sum(lens), heads, kv, d, buckets=buckets)
     want, tol = attention(q, k, v, lens, table=table, far=far, do=do)
     _check_all(_run(q, k, v, do, lens, table, far), want, tol)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("size", [8, 100])
+def test_a_late_key_outweighs_all_before(d, size):
+    """In a tile that all rows see whole: weights against the maximum held
+    so far leave the range, by a little or beyond fp32."""
+    lens = [700]
+    q, k, v, do, _ = _inputs(700, 2, 1, d)
+    k[300] *= size
+    want, tol = attention(q, k, v, lens, do=do)
+    _check_all(_run(q, k, v, do, lens), want, tol)
