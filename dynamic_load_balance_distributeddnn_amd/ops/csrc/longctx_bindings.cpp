@@ -150,7 +150,8 @@ static std::vector<Tensor> packed_attn_fwd(Tensor q, Tensor k, Tensor v,
   return {o, stats};
 }
 
-// -> dq, dk, dv and, with a table and `table_grad`, its gradient.
+// work_kv: the key tiles in steps of 64 queries for heads of up to 64, of
+// 32 for others.  -> dq, dk, dv and, with a table and `table_grad`, its gradient.
 static std::vector<Tensor> packed_attn_bwd(
     Tensor q, Tensor k, Tensor v, Tensor o, Tensor stats, Tensor go,
     WorkList work_q, WorkList work_kv, int64_t total, double scale,

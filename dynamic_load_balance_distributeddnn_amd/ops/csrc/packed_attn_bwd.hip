@@ -915,5 +915,6 @@ extern "C" void dlb_packed_attn_bwd(const PaBwd* p, const PaBias* bias,
   if (bias && dtable)
     hipLaunchKernelGGL(pa_table_grad_kernel, dim3(p->H),
                        dim3(PA_TABLE_WAVES * 64), 0, stream, p->part, dtable,
-                       dtable_bf16, (long)p->work_kv.n_chunks, p->H, bias->buckets);
+                       dtable_bf16, (long)p->work_kv.n_chunks, p->H,
+                       bias->buckets);
 }

@@ -248,9 +248,9 @@ pa_fwd_kernel(const PaFwd p, const BiasArg bias) {
   // sum and the output are scaled anew only once the weights of a tile come
   // to more than 2^16, which fp32 and the bf16 weights (their step is
   // relative) carry without loss.  So no tile looks for its maximum (one of
-  // 8192, 32 heads of 128 over 8: 544 -> 532 us).  False, with nothing done, where
-  // they did; the wave then goes on with any_tile, which has as many
-  // barriers.
+  // 8192, 32 heads of 128 over 8: 544 -> 532 us).  False, with nothing
+  // done, where they did; the wave then goes on with any_tile, which has as
+  // many barriers.
   auto whole_tile = [&](int t) PA_INLINE {
     const int k0 = t * PA_STEP, buf = t & 1;
     const bool more = t + 1 < it.end;

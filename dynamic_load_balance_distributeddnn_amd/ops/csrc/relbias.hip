@@ -358,12 +358,12 @@ extern "C" void dlb_relbias_fwd(const void* table, void* out,
 // diagonals, workgroups of a head.  n: elements of a vector.
 static void rb_bwd_shape(const RbArgs& a, int n, int* rows, long* strips,
                          long* blocks) {
-  // About 3072 waves: 4096 run at a time, and a last few alone would cost
+  // About 12 waves a CU: 16 run at a time, and a last few alone would cost
   // as much as the first.  32 heads of 4096 x 4096 in bf16: 219 us (4.9
   // TB/s), with 64 rows a wave 270; 16 of 2047 x 2047: 45, with twice the
   // waves 55.
   const long span = 64 * n;
-  const long all = (a.H * rb_div(a.K, span) * a.Q / 3072 + 8) / 8 * 8;
+  const long all = (a.H * rb_div(a.K, span) * a.Q / (12 * 256) + 8) / 8 * 8;
   *rows = (int)(all > 512 ? 512 : all);
   *strips = rb_div(a.K + *rows - 1, span);
   *blocks = rb_div(*strips * rb_div(a.Q, *rows), 4);

@@ -97,13 +97,13 @@ class PackedSequences:
         limit fill the places decides: the limit is the best of a few by
         what their launch and join take, in steps.  A chunk costs 8 of its
         own, a join 2.5 and 0.012 each chunk and head (measured, 1.2 to 2
-        us a step; all for steps of 32 rows).  Backward in us, with limits of a share of the whole by
-        384, 512, 640 and 768, the one taken last: one of 8192, 16 heads of
-        64 over 4, 621, 572, 560, 623 (640); five of 4096 in all, 16 heads
-        of 64 with a bias, 114, 118, 126, 125 (384); one of 8192, 32 heads
-        of 128 over 8, 2109, 2040, 1968, 1912 (768).  Below 12 steps chunks
-        lose: eight of 512, 16 heads of 128 over 4, 102 us with 8, 91 with
-        12, 98 with 16.
+        us a step; all for steps of 32 rows).  Backward in us, with limits
+        of a share of the whole by 384, 512, 640 and 768, and the one taken:
+        one of 8192, 16 heads of 64 over 4, 621, 572, 560, 623 (640); five
+        of 4096 in all, 16 heads of 64 with a bias, 114, 118, 126, 125
+        (384); one of 8192, 32 heads of 128 over 8, 2109, 2040, 1968, 1912
+        (768).  Below 12 steps chunks lose: eight of 512, 16 heads of 128
+        over 4, 102 us with 8, 91 with 12, 98 with 16.
         """
         seq, tile = self._tiles()
         steps = (-(-(self._n[seq] - tile * TILE_ROWS) // rows)

@@ -103,13 +103,15 @@ def test_plain_bias(both):
 @pytest.mark.parametrize("lens", [
     [5, 0, TILE_ROWS, TILE_ROWS + 1, 1000], [1], [], [9000],
     [3000, 1, 2500, 300, 77]])
-def test_work_lists(lens, heads, kv):
+@pytest.mark.parametrize("tile_rows,at_once", [(32, 512), (64, 768)])
+def test_work_lists(lens, heads, kv, tile_rows, at_once):
     """Every step of every tile is in one chunk, the longest chunks come
     first, and the chunks of a cut tile have places of their own next to
     each other, which its join names."""
     pack = FD.PackedSequences(torch.tensor(lens, dtype=torch.long))
     assert pack.total == sum(lens) and len(pack) == len(lens)
-    for keys, (rows, n, slots) in enumerate(pack.host_work(heads, kv)):
+    for keys, (rows, n, slots) in enumerate(
+            pack.host_work(heads, kv, tile_rows, at_once)):
         chunks, joins = rows[:n].tolist(), rows[n:].tolist()
         size = [c[4] - c[3] for c in chunks]
         assert size == sorted(size, reverse=True)
@@ -122,7 +124,7 @@ def test_work_lists(lens, heads, kv):
         for (first, length) in zip(pack.offsets, lens):
             for tile in range(-(-length // TILE_ROWS)):
                 if keys:
-                    want = -(-(length - tile * TILE_ROWS) // 32)
+                    want = -(-(length - tile * TILE_ROWS) // tile_rows)
                     want *= heads // kv
                 else:
                     want = -(-min((tile + 1) * TILE_ROWS, length) // 64)
