@@ -6,7 +6,7 @@ Both are plain host-side descriptions; nothing here reads a device.
 from __future__ import annotations
 
 import math
-from functools import lru_cache
+from functools import cached_property, lru_cache
 
 import numpy as np
 import torch
@@ -57,6 +57,7 @@ class PackedSequences:
     def __len__(self):
         return len(self.lengths)
 
+    @cached_property
     def _tiles(self):
         """(sequence, tile) of every 128-row tile."""
         tiles = -(-self._n // TILE_ROWS)
@@ -72,7 +73,7 @@ class PackedSequences:
         """A query tile reads the 64-key tiles up to its last row.  Tiles
         with much more to do than a workgroup's share of the whole are cut
         into chunks, whose sums a second kernel joins."""
-        seq, tile = self._tiles()
+        seq, tile = self._tiles
         steps = -(-np.minimum((tile + 1) * TILE_ROWS, self._n[seq]) // 64)
         total = int(steps.sum()) * heads
         # 512 workgroups run at a time, so the longest tile is what a launch
@@ -105,7 +106,7 @@ class PackedSequences:
         (768).  Below 12 steps chunks lose: eight of 512, 16 heads of 128
         over 4, 102 us with 8, 91 with 12, 98 with 16.
         """
-        seq, tile = self._tiles()
+        seq, tile = self._tiles
         steps = (-(-(self._n[seq] - tile * TILE_ROWS) // rows)
                  * (heads // kv_heads))
         longest = int(steps.max()) if len(steps) else 0
@@ -137,13 +138,22 @@ class PackedSequences:
     def _chunks(self, seq, tile, steps, limit):
         """Chunks of at most ``limit`` steps, the longest first, then the
         joins of the tiles that are in several."""
-        parts = -(-steps // max(limit, 1))
+        first = np.asarray(self.offsets[:-1], np.int64)[seq]
+        if not len(steps) or int(steps.max()) <= limit:
+            order = np.argsort(-steps, kind="stable")
+            rows = np.zeros((len(steps), 8), np.int32)
+            rows[:, 0] = first[order]
+            rows[:, 1] = self._n[seq[order]]
+            rows[:, 2] = tile[order]
+            rows[:, 4] = steps[order]
+            rows[:, 5] = -1
+            return rows, len(rows), 0
+        parts = -(-steps // limit)
         which = np.repeat(np.arange(len(steps)), parts)
         part = np.arange(len(which)) - (np.cumsum(parts) - parts)[which]
         cut = parts > 1
         slots = np.cumsum(parts * cut) - parts * cut
         rows = np.zeros((len(which) + int(cut.sum()), 8), np.int32)
-        first = np.asarray(self.offsets[:-1], np.int64)[seq]
         chunks, joins = rows[:len(which)], rows[len(which):]
         chunks[:, 0] = first[which]
         chunks[:, 1] = self._n[seq[which]]
