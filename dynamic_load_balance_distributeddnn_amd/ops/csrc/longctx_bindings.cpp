@@ -10,9 +10,11 @@
 
 extern "C" void dlb_packed_attn_fwd(const PaFwd* p, const PaBias* bias,
                                     int width, hipStream_t stream);
-extern "C" void dlb_packed_attn_bwd(const PaBwd* p, const PaBias* bias,
-                                    int width, void* dtable, int dtable_bf16,
-                                    hipStream_t stream);
+extern "C" void dlb_packed_attn_bwd_q(const PaBwd* p, const PaBias* bias,
+                                      int width, hipStream_t stream);
+extern "C" void dlb_packed_attn_bwd_kv(const PaBwd* p, const PaBias* bias,
+                                       int width, void* dtable,
+                                       int dtable_bf16, hipStream_t stream);
 extern "C" void dlb_relbias_fwd(const void* table, void* out, const RbArgs* a,
                                 int size, hipStream_t stream);
 extern "C" long dlb_relbias_bwd_blocks(const RbArgs* a, int size);
@@ -167,51 +169,55 @@ static std::vector<Tensor> packed_attn_bwd(
   PaBwd p{pa_tensor(q, "q"), pa_tensor(k, "k"), pa_tensor(v, "v"),
           pa_tensor(go, "gradient")};
   auto dq = torch::empty({T, H, D}, q.options());
-  auto dk = torch::empty({T, k.size(1), D}, q.options());
-  auto dv = torch::empty_like(dk);
   auto f32 = q.options().dtype(torch::kFloat32);
   auto delta = torch::empty({H, T}, f32);
   p.o = o.data_ptr();
   p.stats = stats.data_ptr<float>();
   p.delta = delta.data_ptr<float>();
   p.dq = dq.data_ptr();
-  p.dk = dk.data_ptr();
-  p.dv = dv.data_ptr();
   p.work_q = pa_work(std::get<0>(work_q), std::get<1>(work_q),
                      std::get<2>(work_q), H, pa_tile(D), q, &keep);
-  p.work_kv = pa_work(std::get<0>(work_kv), std::get<1>(work_kv),
-                      std::get<2>(work_kv), k.size(1), 2 * pa_tile(D), q,
-                      &keep);
   p.H = (int)H;
   p.G = (int)(H / k.size(1));
   p.D = (int)D;
   p.T = T;
   p.scale = (float)scale;
-  std::vector<Tensor> out = {dq, dk, dv};
   PaBias bias{};
+  if (table.has_value()) pa_bias(&bias, *table, H, starts);
+  const PaBias* b = table.has_value() ? &bias : nullptr;
+  const int width = pa_width({p.q, p.k, p.v, p.go}, D);
+  if (p.work_q.n_chunks > 0) {
+    dlb_packed_attn_bwd_q(&p, b, width, current_stream());
+    launched();
+  }
+  // the rest while that runs
+  auto dk = torch::empty({T, k.size(1), D}, q.options());
+  auto dv = torch::empty_like(dk);
+  p.dk = dk.data_ptr();
+  p.dv = dv.data_ptr();
+  p.work_kv = pa_work(std::get<0>(work_kv), std::get<1>(work_kv),
+                      std::get<2>(work_kv), k.size(1), 2 * pa_tile(D), q,
+                      &keep);
+  std::vector<Tensor> out = {dq, dk, dv};
   Tensor part, dtable;
-  if (table.has_value()) {
-    pa_bias(&bias, *table, H, starts);
-    if (table_grad) {
-      part = torch::empty({p.work_kv.n_chunks, H, table->size(0)}, f32);
-      dtable = torch::empty_like(*table);
-      p.part = part.data_ptr<float>();
-      out.push_back(dtable);
-    }
+  if (table.has_value() && table_grad) {
+    part = torch::empty({p.work_kv.n_chunks, H, table->size(0)}, f32);
+    dtable = torch::empty_like(*table);
+    p.part = part.data_ptr<float>();
+    out.push_back(dtable);
+  }
+  if (p.work_kv.n_chunks > 0) {
+    dlb_packed_attn_bwd_kv(&p, b, width,
+                           dtable.defined() ? dtable.data_ptr() : nullptr,
+                           bias.is_bf16, current_stream());
+    launched();
+  } else if (dtable.defined()) {
+    dtable.zero_();
   }
   if (total < T) {
     dq.slice(0, total).zero_();
     dk.slice(0, total).zero_();
     dv.slice(0, total).zero_();
-  }
-  if (p.work_q.n_chunks > 0) {
-    dlb_packed_attn_bwd(&p, table.has_value() ? &bias : nullptr,
-                        pa_width({p.q, p.k, p.v, p.go}, D),
-                        dtable.defined() ? dtable.data_ptr() : nullptr,
-                        bias.is_bf16, current_stream());
-    launched();
-  } else if (dtable.defined()) {
-    dtable.zero_();
   }
   return out;
 }

@@ -874,14 +874,10 @@ pa_table_grad_kernel(const float* __restrict__ part, void* out, int is_bf16,
 }
 
 template <int DP, int W>
-static void pa_bwd_go(const PaBwd& p, const PaBias* bias,
-                      hipStream_t stream) {
-  const unsigned H = p.H, kvh = p.H / p.G;
-  const dim3 block(PA_BLOCK);
-  const dim3 grid(p.work_q.n_chunks * H);
-  const dim3 joins(p.work_q.n_joins * H, DP / 32);
-  const dim3 grid_kv(p.work_kv.n_chunks * kvh);
-  const dim3 joins_kv(p.work_kv.n_joins * kvh, DP / 16);
+static void pa_bwd_q_go(const PaBwd& p, const PaBias* bias,
+                        hipStream_t stream) {
+  const dim3 block(PA_BLOCK), grid((unsigned)p.work_q.n_chunks * p.H);
+  const dim3 joins((unsigned)p.work_q.n_joins * p.H, DP / 32);
   if (bias)
     hipLaunchKernelGGL((pa_bwd_q_kernel<DP, W, true, PaBias>), grid, block, 0,
                        stream, p, *bias);
@@ -891,27 +887,47 @@ static void pa_bwd_go(const PaBwd& p, const PaBias* bias,
   if (joins.x)
     hipLaunchKernelGGL((pa_bwd_q_join_kernel<DP, W>), joins, block, 0, stream,
                        p);
+}
+
+template <int DP, int W>
+static void pa_bwd_kv_go(const PaBwd& p, const PaBias* bias,
+                         hipStream_t stream) {
+  const unsigned kvh = p.H / p.G;
+  const dim3 block(PA_BLOCK), grid(p.work_kv.n_chunks * kvh);
+  const dim3 joins(p.work_kv.n_joins * kvh, DP / 16);
   if (bias)
-    hipLaunchKernelGGL((pa_bwd_kv_kernel<DP, W, true, PaBias>), grid_kv,
-                       block, 0, stream, p, *bias);
+    hipLaunchKernelGGL((pa_bwd_kv_kernel<DP, W, true, PaBias>), grid, block,
+                       0, stream, p, *bias);
   else
-    hipLaunchKernelGGL((pa_bwd_kv_kernel<DP, W, false, PaNoBias>), grid_kv,
+    hipLaunchKernelGGL((pa_bwd_kv_kernel<DP, W, false, PaNoBias>), grid,
                        block, 0, stream, p, PaNoBias{});
-  if (joins_kv.x)
-    hipLaunchKernelGGL((pa_bwd_kv_join_kernel<DP, W>), joins_kv, block, 0,
+  if (joins.x)
+    hipLaunchKernelGGL((pa_bwd_kv_join_kernel<DP, W>), joins, block, 0,
                        stream, p);
 }
 
-// width: as in the forward.
-extern "C" void dlb_packed_attn_bwd(const PaBwd* p, const PaBias* bias,
-                                    int width, void* dtable, int dtable_bf16,
-                                    hipStream_t stream) {
-  auto go = [&](auto go64, auto go128) {
-    (p->D <= 64 ? go64 : go128)(*p, bias, stream);
-  };
-  if (width == 16) go(pa_bwd_go<64, 16>, pa_bwd_go<128, 16>);
-  else if (width == 4) go(pa_bwd_go<64, 4>, pa_bwd_go<128, 4>);
-  else go(pa_bwd_go<64, 2>, pa_bwd_go<128, 2>);
+#define PA_BWD_GO(GO)                                   \
+  {                                                     \
+    auto go = [&](auto go64, auto go128) {              \
+      (p->D <= 64 ? go64 : go128)(*p, bias, stream);    \
+    };                                                  \
+    if (width == 16) go(GO<64, 16>, GO<128, 16>);       \
+    else if (width == 4) go(GO<64, 4>, GO<128, 4>);     \
+    else go(GO<64, 2>, GO<128, 2>);                     \
+  }
+
+// The two halves, so that the host can go on with the second's results
+// while the first runs.  Queries: dq and delta.  width: as in the forward.
+extern "C" void dlb_packed_attn_bwd_q(const PaBwd* p, const PaBias* bias,
+                                      int width, hipStream_t stream) {
+  PA_BWD_GO(pa_bwd_q_go)
+}
+
+// Keys, behind the queries: dk, dv and the table's gradient.
+extern "C" void dlb_packed_attn_bwd_kv(const PaBwd* p, const PaBias* bias,
+                                       int width, void* dtable,
+                                       int dtable_bf16, hipStream_t stream) {
+  PA_BWD_GO(pa_bwd_kv_go)
   if (bias && dtable)
     hipLaunchKernelGGL(pa_table_grad_kernel, dim3(p->H),
                        dim3(PA_TABLE_WAVES * 64), 0, stream, p->part, dtable,
