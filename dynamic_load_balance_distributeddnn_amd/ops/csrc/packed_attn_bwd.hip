@@ -35,8 +35,12 @@
 #include "packed_attn.h"
 
 // ---- The table's gradient: sums of dS along its diagonals, then of the
-// diagonals of a bucket, all in a fixed order.  The last bucket is left
-// out: a row's dS sum to 0, so it is minus the sum of the others.
+// diagonals of a bucket, all in a fixed order.  The last bucket, which has
+// no end, a lane sums by itself (`far`).  A row's dS sum to 0, but minus the
+// sum of the other buckets would leave their rounding where no pair has the
+// last one or its weights are 0.  What that costs, backward and forward: five
+// of 4096 in all, 16 heads of 64, 142 -> 144 us; one of 8192, 16 heads of 128
+// over 2, 1511 -> 1598, of which the heads' order (see the kernel) is 35.
 #define PA_DISTANCES 512  // with that many sums a wave
 #define PA_FARHEADS 32    // of a group that LDS keeps the far bias of
 
@@ -73,13 +77,14 @@ __device__ PA_INLINE void pa_diagonals(const f32x16& ds, float& a, float& b,
 // of an addition meet.
 __device__ PA_INLINE void pa_add_diagonals(const f32x16& ds, int n0,
                                            int far_from, float* sums,
-                                           int lane) {
-  const int x = lane & 31;
+                                           float& far, int lane) {
+  const int n = n0 + 4 * (lane >> 5) - (lane & 31);
   float a, b;
-  pa_diagonals(ds, a, b, x);
+  pa_diagonals(ds, a, b, lane & 31);
+  if (n >= far_from) far += a;
+  if (n + 32 >= far_from) far += b;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const int n = n0 + 4 * h - x;
     if ((lane >> 5) == h) {
       if (n >= 0 && n < far_from)
         __hip_atomic_fetch_add(sums + n, a, __ATOMIC_RELAXED,
@@ -112,7 +117,7 @@ __device__ PA_INLINE void pa_add_buckets(const f32x16& ds, int n0,
       if (z >= off && pb == b) v += pv;
     }
     const int nb = __shfl_up(b, 1, 64);
-    const bool last = b >= 0 && b < buckets - 1 && (z == 31 || nb != b);
+    const bool last = b >= 0 && (z == 31 || nb != b);
     if (last && lane < 32) sums[b] += v;
     if (last && lane >= 32) sums[b] += v;
   }
@@ -463,6 +468,7 @@ pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
   __shared__ unsigned char s_bucket[BIAS ? PA_DISTANCES : 1];
   // sums of each wave by distance, or by bucket where far_from is larger
   __shared__ float s_sums[BIAS ? 4 : 1][BIAS ? PA_DISTANCES : 1];
+  __shared__ float s_far_sum[BIAS ? 4 : 1];
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -485,10 +491,10 @@ pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
   // The order of the steps: first the tiles that need neither a mask nor
   // the table's sums, from the sequence's end backwards and every head of
   // a tile in turn, so that the workgroups of a sequence read the same
-  // queries at the same time, from L2; then the others, head by head.
+  // queries at the same time, from L2; then the others, head by head (with
+  // the table's sums all of them).
   int other = min(PA_ROWS / ROWS, nt);  // tiles of the second part
-  if (BIAS && p.part)
-    other = min(max(other, (far_from + PA_ROWS + ROWS - 1) / ROWS), nt);
+  if (BIAS && p.part) other = nt;
   const int h0 = hk * p.G, bulk = (nt - other) * p.G;
   // tile and head of a step
   auto tile_of = [&](int s) PA_INLINE {
@@ -651,17 +657,28 @@ pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
       }
     }
   };
+  float far_sum = 0.f;  // this lane's part of the last bucket
   auto table_sums = [&](const f32x16& dp, int q0) PA_INLINE {
     if constexpr (BIAS) {
+      if (!p.part) return;
       const int n0 = q0 - w0;  // distance of diagonal 0
-      if (p.part && n0 - 31 < far_from) {
-        f32x16 mine = dp;
-        if (key >= len) mine = pa_zero16();
-        if (far_from <= PA_DISTANCES)
-          pa_add_diagonals(mine, n0, far_from, s_sums[wave], lane);
-        else
-          pa_add_buckets(mine, n0, s_start, bias.buckets, s_sums[wave],
-                         lane);
+      f32x16 mine = dp;
+      if (key >= len) mine = pa_zero16();
+      // rows behind the sequence have weights of 0, but repeat a row that
+      // may hold no numbers
+      if (q0 + 31 >= len)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (q0 + 8 * (r >> 2) + 4 * half + (r & 3) >= len) mine[r] = 0.f;
+      if (n0 - 31 >= far_from) {
+        float sum[4] = {};
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sum[r & 3] += mine[r];
+        far_sum += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      } else if (far_from <= PA_DISTANCES) {
+        pa_add_diagonals(mine, n0, far_from, s_sums[wave], far_sum, lane);
+      } else {
+        pa_add_buckets(mine, n0, s_start, bias.buckets, s_sums[wave], lane);
       }
     }
   };
@@ -757,15 +774,18 @@ pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
     while (step < stop) go(any_tile);
     if constexpr (BIAS) {
       if (p.part) {
+        far_sum = wave_reduce_sum(far_sum);
+        if (lane == 0) s_far_sum[wave] = far_sum;
+        far_sum = 0.f;
         __syncthreads();
         float* out = p.part + (chunk * p.H + h0 + head) * bias.buckets;
         const bool by_distance = far_from <= PA_DISTANCES;
         // eight threads a bucket
         for (int b = threadIdx.x >> 3; b < bias.buckets; b += PA_BLOCK / 8) {
           const int from = by_distance ? s_start[b] : b;
-          const int to = b == bias.buckets - 1 ? from
-                         : by_distance         ? s_start[b + 1]
-                                               : b + 1;
+          const int to = !by_distance              ? b + 1
+                         : b + 1 < bias.buckets ? s_start[b + 1]
+                                                : from;
           float v = 0.f;
           for (int n = from + (threadIdx.x & 7); n < to; n += 8)
             v += (s_sums[0][n] + s_sums[1][n]) +
@@ -773,6 +793,9 @@ pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
           v += __shfl_xor(v, 1, 64);
           v += __shfl_xor(v, 2, 64);
           v += __shfl_xor(v, 4, 64);
+          if (b == bias.buckets - 1)
+            v += (s_far_sum[0] + s_far_sum[1]) +
+                 (s_far_sum[2] + s_far_sum[3]);
           if ((threadIdx.x & 7) == 0) out[b] = v;
         }
         __syncthreads();
@@ -784,9 +807,9 @@ pa_bwd_kv_kernel(const PaBwd p, const BiasArg bias) {
   }
   if constexpr (BIAS) {
     if (p.part) {  // heads that only other chunks have sums for
-      const int g_end = it.end > bulk ? (it.end - 1 - bulk) / other : -1;
+      const int g_end = (it.end - 1) / other;
       for (int x = 0; x < p.G; ++x)
-        if (it.end <= bulk || x < g_first || x > g_end)
+        if (x < g_first || x > g_end)
           for (int b = threadIdx.x; b < bias.buckets; b += PA_BLOCK)
             p.part[(chunk * p.H + h0 + x) * bias.buckets + b] = 0.f;
     }
@@ -837,7 +860,6 @@ __global__ void __launch_bounds__(PA_TABLE_WAVES * 64)
 pa_table_grad_kernel(const float* __restrict__ part, void* out, int is_bf16,
                      long chunks, int H, int buckets) {
   __shared__ float s_part[PA_TABLE_WAVES][64];
-  __shared__ float s_sum[PA_MAXBUCKETS];
   const int h = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   for (int b0 = 0; b0 < buckets; b0 += 64) {
     const int b = min(b0 + lane, buckets - 1);
@@ -851,25 +873,17 @@ pa_table_grad_kernel(const float* __restrict__ part, void* out, int is_bf16,
       }
     s_part[wave][lane] = (v[0] + v[1]) + (v[2] + v[3]);
     __syncthreads();
-    if (wave == 0) {
+    if (wave == 0 && b0 + lane < buckets) {
       float x = 0.f;
 #pragma unroll
       for (int w = 0; w < PA_TABLE_WAVES; ++w) x += s_part[w][lane];
-      if (b0 + lane < buckets) s_sum[b0 + lane] = x;
+      const long at = (long)b * H + h;
+      if (is_bf16)
+        static_cast<__bf16*>(out)[at] = (__bf16)x;
+      else
+        static_cast<float*>(out)[at] = x;
     }
     __syncthreads();
-  }
-  if (wave > 0) return;
-  float all = 0.f;
-  for (int b = lane; b < buckets - 1; b += 64) all += s_sum[b];
-  all = __shfl(wave_reduce_sum(all), 0, 64);
-  for (int b = lane; b < buckets; b += 64) {
-    const float x = b < buckets - 1 ? s_sum[b] : -all;
-    const long at = (long)b * H + h;
-    if (is_bf16)
-      static_cast<__bf16*>(out)[at] = (__bf16)x;
-    else
-      static_cast<float*>(out)[at] = x;
   }
 }
 

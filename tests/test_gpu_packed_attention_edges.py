@@ -1,0 +1,160 @@
+"""Packed causal attention where single entries of its results can go wrong:
+the far bucket's gradient, exactness of the keys'."""
+
+import math
+
+import pytest
+import torch
+
+from longctx_reference import SECOND, SLACK, U, bucket_by_count, check
+
+pytestmark = pytest.mark.gpu
+
+
+def _fd():
+    from dynamic_load_balance_distributeddnn_amd.ops import functional as FD
+    return FD
+
+
+def _inputs(rows, heads, kv, d, seed=0, buckets=0, table_type=torch.float32):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+
+    def normal(*shape, dtype=torch.bfloat16):
+        return torch.randn(*shape, device="cuda", generator=gen).to(dtype)
+
+    q, k, v = normal(rows, heads, d), normal(rows, kv, d), normal(rows, kv, d)
+    do = normal(rows, heads, d)
+    table = normal(buckets, heads, dtype=table_type) if buckets else None
+    return q, k, v, do, table
+
+
+def _run(q, k, v, do, lens, table=None, far=128):
+    """All outputs by name."""
+    FD = _fd()
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    extra = {}
+    if table is not None:
+        leaves.append(table.detach().requires_grad_())
+        extra = dict(bias_table=leaves[3], max_distance=far)
+    o = FD.packed_causal_attention(
+        *leaves[:3], FD.PackedSequences(lens, device=q.device), **extra)
+    grads = torch.autograd.grad(o, leaves, do)
+    return dict(zip(("o", "dq", "dk", "dv", "dtable"),
+                    (o.detach(), *grads)))
+
+
+def _exact_delta(q, k, v, lens, do, table=None, far=128):
+    """dK and the table's gradient in 64 bits, with bounds in which delta
+    has no part: it is exact to fp32 there.
+
+    A weight and its gradient are off by SLACK of the sums without signs
+    (see the reference); dK's operand dS is rounded to bf16 once, the
+    result once; the table's gradient is a sum in fp32 of each bucket's own
+    pairs, so no other bucket is in its bound.
+    """
+    q, k, v, do = (t.detach().double() for t in (q, k, v, do))
+    heads, d = q.shape[1:]
+    group = heads // k.shape[1]
+    val = {"dk": torch.zeros_like(k)}
+    tol = {"dk": torch.zeros_like(k)}
+    last_step = 2.0 ** -24
+    if table is not None:
+        last_step = U if table.dtype == torch.bfloat16 else last_step
+        table = table.detach().double()
+        val["dtable"] = torch.zeros_like(table)
+        tol["dtable"] = torch.zeros_like(table)
+        by = torch.tensor([bucket_by_count(n, table.shape[0], far)
+                           for n in range(max(lens))], device=q.device)
+    first = 0
+    for n in lens:
+        at = slice(first, first + n)
+        first += n
+        i = torch.arange(n, device=q.device)
+        gap = i[:, None] - i
+        for h in range(heads):
+            g = h // group
+            s = q[at, h] @ k[at, g].T * d ** -0.5
+            if table is not None:
+                which = by[gap.clamp(min=0)]
+                s = s + table[:, h][which]
+            s = s.masked_fill(gap < 0, -math.inf)
+            top = s.amax(-1, keepdim=True)
+            p = torch.exp(s - top.masked_fill(top == -math.inf, 0))
+            total = p.sum(-1, keepdim=True)
+            p = p / total.masked_fill(total == 0, 1)
+            o, dh, vh = p @ v[at, g], do[at, h], v[at, g]
+            ds = p * (dh @ vh.T - (dh * o).sum(-1, keepdim=True))
+            e = SLACK * p * (dh.abs() @ vh.abs().T
+                             + (dh * o).abs().sum(-1, keepdim=True))
+            qh = q[at, h] * d ** -0.5
+            val["dk"][at, g] += ds.T @ qh
+            tol["dk"][at, g] += (U * ds.abs() + e).T @ qh.abs()
+            if table is not None:
+                for b in range(table.shape[0]):
+                    there = (which == b) & (gap >= 0)
+                    val["dtable"][b, h] += ds[there].sum()
+                    tol["dtable"][b, h] += e[there].sum()
+    tol["dk"] = SECOND * (tol["dk"] + U * val["dk"].abs())
+    if table is not None:
+        tol["dtable"] = SECOND * (tol["dtable"]
+                                  + last_step * val["dtable"].abs())
+    return val, tol
+
+
+# ------------------------------------------------ the far bucket's gradient
+@pytest.mark.parametrize("lens,far", [([35] * 20, 128), ([100, 64, 1], 128),
+                                      ([300, 900], 2000)])
+@pytest.mark.parametrize("heads,kv,d", [(4, 4, 64), (4, 2, 100)])
+def test_a_bucket_that_no_pair_reaches_has_no_gradient(lens, far, heads, kv,
+                                                       d):
+    buckets = 32
+    q, k, v, do, table = _inputs(sum(lens), heads, kv, d, buckets=buckets)
+    reached = {bucket_by_count(n, buckets, far) for n in range(max(lens))}
+    out = [b for b in range(buckets) if b not in reached]
+    assert buckets - 1 in out
+    got = _run(q, k, v, do, lens, table, far)["dtable"]
+    assert bool((got[out] == 0).all()), got[out]
+
+
+@pytest.mark.parametrize("low", [-math.inf, -1e4,
+                                 torch.finfo(torch.float32).min])
+@pytest.mark.parametrize("lens,far", [([700, 40], 128), ([2500], 2000)])
+def test_a_far_bucket_that_masks_has_no_gradient(low, lens, far):
+    """A row has a weight at distance 0, so what the far bucket takes out
+    has one of 0, and 0 is its sum."""
+    q, k, v, do, table = _inputs(sum(lens), 4, 2, 64, buckets=32)
+    table[31] = low
+    got = _run(q, k, v, do, lens, table, far)
+    assert bool((got["dtable"][31] == 0).all()), got["dtable"][31]
+    want, tol = _exact_delta(q, k, v, lens, do, table, far)
+    for name in want:
+        check(got[name], want[name], tol[name], name)
+
+
+@pytest.mark.parametrize("row", [20, 34])
+def test_a_gradient_that_is_no_number_stays_in_its_buckets(row):
+    """The first sequence does not reach the far bucket, the second does.
+    Its last row is what the tile repeats behind the sequence."""
+    lens = [35, 300]
+    q, k, v, do, table = _inputs(335, 2, 2, 64, buckets=32)
+    want, tol = _exact_delta(q[35:], k[35:], v[35:], [300], do[35:], table)
+    do[row] = math.nan
+    got = _run(q, k, v, do, lens, table)["dtable"]
+    far = [b for b in range(32) if bucket_by_count(35, 32, 128) < b]
+    assert 31 in far and bool(torch.isnan(got[0]).all())
+    check(got[far], want["dtable"][far], tol["dtable"][far], "dtable")
+
+
+@pytest.mark.parametrize("lens,heads,kv,d,far", [
+    ([130, 1, 64], 4, 2, 100, 128), ([600, 300], 2, 2, 128, 128),
+    ([2500, 900, 33], 4, 2, 64, 128), ([2500, 900, 33], 4, 1, 64, 2000),
+    ([3000], 2, 2, 128, 300), ([1500], 40, 1, 32, 64)])
+@pytest.mark.parametrize("buckets", [2, 32])
+def test_keys_and_table_gradients_are_exact_in_delta(lens, heads, kv, d, far,
+                                                     buckets):
+    """Each bucket by its own pairs; sequences whose lists are cut too."""
+    q, k, v, do, table = _inputs(sum(lens), heads, kv, d, buckets=buckets)
+    want, tol = _exact_delta(q, k, v, lens, do, table, far)
+    got = _run(q, k, v, do, lens, table, far)
+    for name in want:
+        check(got[name], want[name], tol[name], name)
