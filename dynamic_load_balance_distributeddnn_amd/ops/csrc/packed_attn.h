@@ -372,9 +372,13 @@ __device__ inline float pa_bias(unsigned entry, int is_bf16) {
   const float y = x * PA_LOG2E;
   return finite ? fminf(fmaxf(y, -1e37f), 1e37f) : y;
 }
-// Whether a tile's one bias can be added outside of the exponent's fma:
-// beyond, a score has to drown in it first.
-__device__ inline bool pa_moderate(float x) { return fabsf(x) <= 1e30f; }
+// Whether a tile's one bias can be added outside of the scores' fma, to the
+// maximum that is taken off them: that is the sum with a score, and what the
+// sum's rounding drops of the score stays in the exponent.  Up to 2^14 that
+// is 2^-11 at most, a tenth of the weights' own step in bf16; beyond 2^30 it
+// could be the score itself, without a maximum taken off.  There each score
+// is rounded with the bias before the maximum is.
+__device__ inline bool pa_moderate(float x) { return fabsf(x) <= 16384.f; }
 
 __device__ inline const __bf16* pa_at(const PaTensor& t, long row, int head) {
   return static_cast<const __bf16*>(t.p) + row * t.row + head * t.head;

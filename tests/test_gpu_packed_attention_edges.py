@@ -1,12 +1,14 @@
 """Packed causal attention where single entries of its results can go wrong:
-the far bucket's gradient, exactness of the keys'."""
+the far bucket's gradient, exactness of the keys', biases that drown the
+scores."""
 
 import math
 
 import pytest
 import torch
 
-from longctx_reference import SECOND, SLACK, U, bucket_by_count, check
+from longctx_reference import (SECOND, SLACK, U, attention, bucket_by_count,
+                               check)
 
 pytestmark = pytest.mark.gpu
 
@@ -158,3 +160,45 @@ def test_keys_and_table_gradients_are_exact_in_delta(lens, heads, kv, d, far,
     got = _run(q, k, v, do, lens, table, far)
     for name in want:
         check(got[name], want[name], tol[name], name)
+
+
+# ------------------------------------------ a finite far bias, large scores
+@pytest.mark.parametrize("low", [-1e5, -1e10, -1e20])
+@pytest.mark.parametrize("length,heads", [(600, 2), (2500, 2), (600, 16)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_far_bias_that_drowns_large_scores(low, length, heads, d):
+    """The first hundred keys have scores of some hundreds and are seen by
+    rows far enough behind through the far bucket alone."""
+    q, k, v, do, table = _inputs(length, heads, heads, d, buckets=32)
+    k[:100] *= 60
+    table[31] = low
+    want, tol = attention(q, k, v, [length], table=table, do=do)
+    got = _run(q, k, v, do, [length], table)
+    for name, t in got.items():
+        assert bool(torch.isfinite(t).all()), name
+    for name in ("o", "dq"):  # rows that do not see them otherwise
+        check(got[name][230:], want[name][230:], tol[name][230:], name)
+    for name in ("dk", "dv"):  # keys that no other row sees
+        check(got[name][230:], want[name][230:], tol[name][230:], name)
+
+
+@pytest.mark.parametrize("high", [300.0, 1e4])
+def test_far_bias_that_outweighs_all(high):
+    """Rows that reach the far bucket weigh its keys alone: their scores
+    are rounded at the bias's size, 2**-11 at most as exponents of 2."""
+    q, k, v, do, table = _inputs(700, 2, 2, 64, buckets=32)
+    table[31] = high
+    want, tol = attention(q, k, v, [700], table=table, do=do)
+    got = _run(q, k, v, do, [700], table)
+    assert all(bool(torch.isfinite(t).all()) for t in got.values())
+    first = next(n for n in range(200) if bucket_by_count(n, 32, 128) == 31)
+    rows = slice(first + 1, 700)
+    # a weight is off by 2 ** 2**-11 of itself, its row's sum too
+    room = 2 * (2.0 ** (2.0 ** -11) - 1)
+    for h in range(2):
+        i = torch.arange(700, device="cuda")
+        s = q[:, h].double() @ k[:, h].double().T / 8
+        s = s.masked_fill(i[:, None] - i < first, -math.inf)[rows]
+        p = torch.softmax(s, -1) @ v[:, h].double().abs()
+        check(got["o"][rows, h], want["o"][rows, h],
+              tol["o"][rows, h] + room * p, "o")
