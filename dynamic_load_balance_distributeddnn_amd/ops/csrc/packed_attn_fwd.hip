@@ -231,7 +231,10 @@ pa_fwd_kernel(const PaFwd p, const BiasArg bias) {
           if (j * 32 + 8 * (r >> 2) + (r & 3) > lim) s[j][r] = -INFINITY;
       const float top = maximum(s);
       const float ref = top == -INFINITY ? 0.f : top;
-      const float f = __builtin_amdgcn_exp2f(m - ref);
+      // before the first weight there is nothing to scale but infinities that
+      // were taken out of the values: 0 of those would be NaN
+      const float f =
+          m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - ref);
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll

@@ -1,6 +1,6 @@
 """Packed causal attention where single entries of its results can go wrong:
 the far bucket's gradient, exactness of the keys', biases that drown the
-scores."""
+scores, infinities that a row does see."""
 
 import math
 
@@ -202,3 +202,25 @@ def test_far_bias_that_outweighs_all(high):
         p = torch.softmax(s, -1) @ v[:, h].double().abs()
         check(got["o"][rows, h], want["o"][rows, h],
               tol["o"][rows, h] + room * p, "o")
+
+
+# ------------------------------------------- infinities that a row does see
+@pytest.mark.parametrize("value", [math.inf, -math.inf])
+@pytest.mark.parametrize("length,at", [(150, 5), (150, 70), (150, 129),
+                                       (2500, 3), (2500, 2470)])
+@pytest.mark.parametrize("biased", [False, True])
+def test_an_infinite_value_stays_one_for_the_rows_that_see_it(value, length,
+                                                              at, biased):
+    lens = [40, length, 45]
+    rows = sum(lens)
+    q, k, v, do, table = _inputs(rows, 2, 1, 64,
+                                 buckets=32 if biased else 0)
+    want, tol = attention(q, k, v, lens, table=table)
+    v[40 + at, :, 3:] = value
+    got = _run(q, k, v, do, lens, table)["o"]
+    sees = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    sees[40 + at:40 + length] = True
+    assert bool((got[sees][..., 3:] == value).all())
+    check(got[sees][..., :3], want["o"][sees][..., :3],
+          tol["o"][sees][..., :3], "beside it")
+    check(got[~sees], want["o"][~sees], tol["o"][~sees], "not seen")
