@@ -118,8 +118,12 @@ __device__ PA_INLINE void pa_add_buckets(const f32x16& ds, int n0,
     }
     const int nb = __shfl_up(b, 1, 64);
     const bool last = b >= 0 && (z == 31 || nb != b);
-    if (last && lane < 32) sums[b] += v;
-    if (last && lane >= 32) sums[b] += v;
+    // a bucket can end in both halves
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (last && (lane >> 5) == h)
+        __hip_atomic_fetch_add(sums + b, v, __ATOMIC_RELAXED,
+                               __HIP_MEMORY_SCOPE_WORKGROUP);
   }
 }
 

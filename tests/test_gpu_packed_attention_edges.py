@@ -162,6 +162,20 @@ def test_keys_and_table_gradients_are_exact_in_delta(lens, heads, kv, d, far,
         check(got[name], want[name], tol[name], name)
 
 
+@pytest.mark.parametrize("lens,heads,kv", [([700, 40], 4, 2),
+                                           ([2500], 2, 2)])
+def test_one_bucket_for_both_halves_of_a_block(lens, heads, kv):
+    """Distances 1 to 999 are one bucket: both halves of a wave add to it
+    in every block."""
+    q, k, v, do, table = _inputs(sum(lens), heads, kv, 64, buckets=3)
+    assert bucket_by_count(999, 3, 10 ** 6) == 1
+    want, tol = _exact_delta(q, k, v, lens, do, table, 10 ** 6)
+    got = _run(q, k, v, do, lens, table, 10 ** 6)
+    check(got["dtable"], want["dtable"], tol["dtable"], "dtable")
+    again = _run(q, k, v, do, lens, table, 10 ** 6)
+    assert torch.equal(got["dtable"], again["dtable"])
+
+
 # ------------------------------------------ a finite far bias, large scores
 @pytest.mark.parametrize("low", [-1e5, -1e10, -1e20])
 @pytest.mark.parametrize("length,heads", [(600, 2), (2500, 2), (600, 16)])
