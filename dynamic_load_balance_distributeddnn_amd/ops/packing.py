@@ -45,7 +45,7 @@ class PackedSequences:
         n = n.astype(np.int64)
         if (n < 0).any():
             raise ValueError("lengths must not be negative")
-        if int(n.sum()) >= 2 ** 30:
+        if sum(n.tolist()) >= 2 ** 30:  # whole numbers of any size
             raise ValueError("more than 2**30 - 1 rows in one packing")
         self._n = n
         self.lengths = tuple(n.tolist())
