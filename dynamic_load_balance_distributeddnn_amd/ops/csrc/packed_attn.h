@@ -196,21 +196,26 @@ struct PaFrags {
 // base and tile are the wave's.  Written out because the compiler would let
 // every LDS read, of the other buffer too, wait for the load it knows of.
 // Nobody but s_waitcnt vmcnt(0) and a barrier says that the data is there.
+// The compiler counts no wait states here: the base is copied by a scalar
+// instruction, as a load that reads it too soon after a vector instruction
+// wrote it (a readlane) would not wait for it, and the copy is the state that
+// M0 wants between its write and the load.
 template <int W>
 __device__ inline void pa_to_lds(const __bf16* base, unsigned offset,
                                  __bf16* tile) {
   const unsigned to = (unsigned)(__UINTPTR_TYPE__)(
       (__attribute__((address_space(3))) __bf16*)tile);
+  const __bf16* from;
   if constexpr (W == 16)
     asm volatile(
-        "s_mov_b32 m0, %0\n\ts_nop 0\n\t"
-        "global_load_lds_dwordx4 %1, %2"
-        :: "s"(to), "v"(offset), "s"(base));
+        "s_mov_b32 m0, %1\n\ts_mov_b64 %0, %3\n\t"
+        "global_load_lds_dwordx4 %2, %0"
+        : "=&s"(from) : "s"(to), "v"(offset), "s"(base) : "m0");
   else
     asm volatile(
-        "s_mov_b32 m0, %0\n\ts_nop 0\n\t"
-        "global_load_lds_dword %1, %2"
-        :: "s"(to), "v"(offset), "s"(base));
+        "s_mov_b32 m0, %1\n\ts_mov_b64 %0, %3\n\t"
+        "global_load_lds_dword %2, %0"
+        : "=&s"(from) : "s"(to), "v"(offset), "s"(base) : "m0");
 }
 
 // Brings [ROWS][DP] tiles of one sequence's head slice into LDS, the
