@@ -34,16 +34,21 @@ static void launched() {
   TORCH_CHECK(e == hipSuccess, "kernel launch: ", hipGetErrorString(e));
 }
 
+// Rows are addressed from a tile's first one in 32 bits, 64 at a time.
+static const int64_t PA_MAXSTRIDE = 1 << 24;
+
 static PaTensor pa_tensor(const Tensor& t, const char* name) {
   TORCH_CHECK(t.is_cuda() && t.dim() == 3 &&
                   t.scalar_type() == torch::kBFloat16,
               name, ": a bf16 GPU tensor [rows, heads, size] is wanted");
   TORCH_CHECK(t.size(2) == 1 || t.stride(2) == 1, name,
               ": the last dimension has to be dense");
-  // 64 rows are addressed from one base in 32 bits
-  TORCH_CHECK(t.stride(0) >= 0 && t.stride(0) < (1 << 24) && t.stride(1) >= 0,
-              name, ": row stride out of range");
-  return {t.data_ptr(), t.stride(0), t.stride(1)};
+  // the stride of a single row or head says nothing
+  const int64_t row = t.size(0) > 1 ? t.stride(0) : 0;
+  const int64_t head = t.size(1) > 1 ? t.stride(1) : 0;
+  TORCH_CHECK(row >= 0 && row < PA_MAXSTRIDE && head >= 0, name,
+              ": row stride out of range");
+  return {t.data_ptr(), row, head};
 }
 
 // Bytes a load may have: the head size, the strides and the address are
@@ -327,8 +332,12 @@ static void refuse_eager_inputs(const char* name) {
   }
 }
 
-static Tensor dense_last(const Tensor& t) {
-  return t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous();
+// A tensor the kernels can read: itself, if its strides allow it.
+static Tensor readable(const Tensor& t) {
+  return (t.size(2) == 1 || t.stride(2) == 1) &&
+                 (t.size(0) <= 1 || t.stride(0) < PA_MAXSTRIDE)
+             ? t
+             : t.contiguous();
 }
 
 struct PackedAttention
@@ -338,7 +347,7 @@ struct PackedAttention
                         const MaybeTensor& table0, WorkList work_q,
                         MaybeWork work_kv, int64_t total, double scale,
                         std::vector<int64_t> starts, bool table_grad) {
-    const Tensor q = dense_last(q0), k = dense_last(k0), v = dense_last(v0);
+    const Tensor q = readable(q0), k = readable(k0), v = readable(v0);
     MaybeTensor table;
     if (table0.has_value()) table = table0->contiguous();
     auto out = packed_attn_fwd(q, k, v, work_q, total, scale, table, starts);
@@ -369,7 +378,7 @@ struct PackedAttention
       at::AutoGradMode off(false);
       auto grads = packed_attn_bwd(
           saved[0], saved[1], saved[2], saved[3], saved[4],
-          dense_last(grad[0]), WorkList{saved[6], n[0], n[1]},
+          readable(grad[0]), WorkList{saved[6], n[0], n[1]},
           WorkList{saved[7], n[2], n[3]}, n[4], d["scale"].toDouble(), table,
           d["starts"].toIntVector(), table_grad);
       for (size_t i = 0; i < grads.size(); ++i) out[i] = grads[i];

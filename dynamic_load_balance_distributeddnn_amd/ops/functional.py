@@ -248,7 +248,8 @@ def packed_causal_attention(q, k, v, packing, scale=None, bias_table=None,
     head.  ``packing`` (PackedSequences) says which rows are a sequence;
     a row sees the rows of its own sequence up to itself.  Rows behind the
     last sequence come back as zeros, and so do their gradients.  Views
-    with any row and head strides are read in place.
+    with any head stride and a row stride below 2**24 elements are read in
+    place (others, or those whose last dimension is not dense, are copied).
 
     ``bias_table`` [num_buckets, nhead] adds ``relative_position_bias`` of
     it to the scaled scores without forming the grid; entries of -inf take

@@ -1,6 +1,6 @@
 """Packed causal attention where single entries of its results can go wrong:
 the far bucket's gradient, exactness of the keys', biases that drown the
-scores, infinities that a row does see."""
+scores, infinities that a row does see, rows far apart."""
 
 import math
 
@@ -238,3 +238,23 @@ def test_an_infinite_value_stays_one_for_the_rows_that_see_it(value, length,
     check(got[sees][..., :3], want["o"][sees][..., :3],
           tol["o"][sees][..., :3], "beside it")
     check(got[~sees], want["o"][~sees], tol["o"][~sees], "not seen")
+
+
+# ------------------------------------------------------------- row strides
+@pytest.mark.parametrize("rows,stride", [(3, 2 ** 24), (3, 2 ** 25 + 1),
+                                         (1, 2 ** 40), (1, 77)])
+def test_rows_far_apart(rows, stride):
+    """A row stride that the kernels do not take is copied; the one of a
+    single row says nothing."""
+    q, k, v, do, _ = _inputs(rows, 2, 2, 64)
+    want = _run(q, k, v, do, [rows])
+    room = torch.empty((rows - 1) * stride + 128, dtype=torch.bfloat16,
+                       device="cuda")
+    for turn in range(4):
+        given = [q, k, v, do]
+        far = room.as_strided((rows, 2, 64), (stride, 64, 1))
+        far.copy_(given[turn])
+        given[turn] = far
+        got = _run(*given, [rows])
+        for name in want:
+            assert torch.equal(got[name], want[name]), (turn, name)
