@@ -96,7 +96,8 @@ static PaWork pa_work(const Tensor& list, int64_t chunks, int64_t slots,
                   list.scalar_type() == torch::kInt32 && list.dim() == 2 &&
                   list.size(1) == 8 && chunks >= 0 &&
                   chunks <= list.size(0) && slots >= 0 &&
-                  list.size(0) * heads < (1l << 31),
+                  list.size(0) * heads < (1l << 25) &&
+                  chunks * heads < (1l << 24),  // workgroups of 256
               "packed attention: work list does not fit");
   // the list was made on another stream, maybe: it is not to be used again
   // before this one is done with it

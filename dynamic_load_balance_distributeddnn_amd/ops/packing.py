@@ -14,6 +14,8 @@ import torch
 # Rows of a sequence one workgroup of the attention kernels owns
 # (PA_ROWS in csrc/packed_attn.h).
 TILE_ROWS = 128
+# Workgroups a launch takes: below 2**32 threads, 256 each.
+MAX_WORKGROUPS = 2 ** 24 - 1
 
 
 class PackedSequences:
@@ -28,7 +30,9 @@ class PackedSequences:
     tensors of that device only.
 
     For each head layout it is used with it keeps work lists on the device,
-    of the query tiles and, for gradients, of the key tiles.
+    of the query tiles and, for gradients, of the key tiles.  A list's tiles
+    times the heads have to be below 2**24 (a million sequences of one row
+    with 16 heads are too many).
     """
 
     def __init__(self, lengths, device=None):
@@ -87,7 +91,7 @@ class PackedSequences:
         limit = max(8, total // 384)
         if len(steps) and int(steps.max()) <= 1.75 * total / 512:
             limit = int(steps.max())
-        return self._chunks(seq, tile, steps, limit)
+        return self._chunks(seq, tile, steps, heads, limit)
 
     def _key_work(self, heads, kv_heads, rows, at_once):
         """A key tile is read by the tiles of ``rows`` queries from its
@@ -114,12 +118,12 @@ class PackedSequences:
         least = 12 * 32 // rows
         # many tiles a place: nothing to gain by cutting
         if 2 * longest * at_once <= total or longest <= least:
-            return self._chunks(seq, tile, steps, longest)
+            return self._chunks(seq, tile, steps, kv_heads, longest)
         limits = {max(least, total // n) for n in (384, 512, 640, 768)}
         limit = min(sorted(limits | {longest}),
                     key=lambda x: self._time(steps, kv_heads, x, at_once,
                                              32 / rows))
-        return self._chunks(seq, tile, steps, limit)
+        return self._chunks(seq, tile, steps, kv_heads, limit)
 
     @staticmethod
     def _time(steps, heads, limit, at_once, unit):
@@ -135,9 +139,15 @@ class PackedSequences:
         slots = int((parts * (parts > 1)).sum()) * heads
         return load[-1] + ((2.5 + 0.012 * slots) * unit if slots else 0.0)
 
-    def _chunks(self, seq, tile, steps, limit):
+    def _chunks(self, seq, tile, steps, heads, limit):
         """Chunks of at most ``limit`` steps, the longest first, then the
-        joins of the tiles that are in several."""
+        joins of the tiles that are in several; a workgroup a chunk and
+        head."""
+        parts = -(-steps // max(limit, 1))
+        if int(parts.sum()) * heads > MAX_WORKGROUPS:
+            raise ValueError(f"{int(parts.sum())} tiles of {heads} heads are "
+                             "too many for one launch, 2**24 - 1 in all: use "
+                             "several packings")
         first = np.asarray(self.offsets[:-1], np.int64)[seq]
         if not len(steps) or int(steps.max()) <= limit:
             order = np.argsort(-steps, kind="stable")
@@ -148,7 +158,6 @@ class PackedSequences:
             rows[:, 4] = steps[order]
             rows[:, 5] = -1
             return rows, len(rows), 0
-        parts = -(-steps // limit)
         which = np.repeat(np.arange(len(steps)), parts)
         part = np.arange(len(which)) - (np.cumsum(parts) - parts)[which]
         cut = parts > 1

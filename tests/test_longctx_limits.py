@@ -18,3 +18,16 @@ def test_lengths_whose_sum_leaves_64_bits(lengths):
 
 def test_the_most_rows():
     assert FD.PackedSequences([2 ** 30 - 2, 0, 1]).total == 2 ** 30 - 1
+
+
+def test_more_tiles_than_a_launch_takes():
+    """2**32 threads are one too many: workgroups of 256, one a tile and
+    head."""
+    pack = FD.PackedSequences(np.ones(2 ** 20, np.int64))
+    with pytest.raises(ValueError, match="too many"):
+        pack.host_work(16, 16)
+    with pytest.raises(ValueError, match="too many"):
+        pack.host_work(32, 8)  # the query tiles alone
+    for rows, chunks, slots in pack.host_work(15, 15):
+        assert rows.shape == (2 ** 20, 8)
+        assert (chunks, slots) == (2 ** 20, 0)
