@@ -162,6 +162,21 @@ def test_keys_and_table_gradients_are_exact_in_delta(lens, heads, kv, d, far,
         check(got[name], want[name], tol[name], name)
 
 
+@pytest.mark.parametrize("lens,heads,kv,d", [
+    ([700, 129], 4, 2, 64), ([3000, 200], 2, 1, 128), ([2500], 2, 2, 64)])
+@pytest.mark.parametrize("buckets", [0, 32])
+def test_values_with_a_mean(lens, heads, kv, d, buckets):
+    """delta is large where what it is taken off is the same for all keys:
+    from the stored output it would be off by 2**-8 of that, many times
+    what these bounds have room for (one list is cut, one is not)."""
+    q, k, v, do, table = _inputs(sum(lens), heads, kv, d, buckets=buckets)
+    v = (v.float() * 0.1 + 8).bfloat16()
+    want, tol = _exact_delta(q, k, v, lens, do, table)
+    got = _run(q, k, v, do, lens, table)
+    for name in want:
+        check(got[name], want[name], tol[name], name)
+
+
 @pytest.mark.parametrize("lens,heads,kv", [([700, 40], 4, 2),
                                            ([2500], 2, 2)])
 def test_one_bucket_for_both_halves_of_a_block(lens, heads, kv):
