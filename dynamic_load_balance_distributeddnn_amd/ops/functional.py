@@ -258,13 +258,14 @@ def packed_causal_attention(q, k, v, packing, scale=None, bias_table=None,
     defaults to d ** -0.5.  What a masked position holds, an infinity or
     NaN even, does not reach a row that does not see it.
 
-    On the GPU: bfloat16 (fp32 is cast under autocast), d <= 128; sums,
+    On the GPU: bfloat16 (fp32 is cast to it under autocast, whatever type
+    that names), d <= 128; sums,
     softmax statistics and the gradients' sums are fp32, and results do
     not change from run to run.  The table may be fp32 or bfloat16.
     """
-    if (q.dtype == torch.float32 and q.is_cuda
-            and torch.is_autocast_enabled("cuda")):
-        q, k, v = (t.to(torch.bfloat16) for t in (q, k, v))
+    if q.is_cuda and torch.is_autocast_enabled("cuda"):
+        q, k, v = (t.to(torch.bfloat16) if t.dtype == torch.float32 else t
+                   for t in (q, k, v))
     qs, ks, dtype, device = q.shape, k.shape, q.dtype, q.device
     if not (isinstance(packing, PackedSequences) and len(qs) == 3
             and len(ks) == 3 and ks == v.shape and ks[0] == qs[0]

@@ -1,6 +1,6 @@
 """Packed causal attention where single entries of its results can go wrong:
 the far bucket's gradient, exactness of the keys', biases that drown the
-scores, infinities that a row does see, rows far apart."""
+scores, infinities that a row does see, rows far apart, autocast."""
 
 import math
 
@@ -273,3 +273,23 @@ def test_rows_far_apart(rows, stride):
         got = _run(*given, [rows])
         for name in want:
             assert torch.equal(got[name], want[name]), (turn, name)
+
+
+# ---------------------------------------------------------------- autocast
+@pytest.mark.parametrize("wide", ["q", "k", "v", "kv", "qkv"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_autocast_casts_each_of_the_three(wide, dtype):
+    """To bfloat16, the kernels' one type, whatever type autocast names."""
+    FD = _fd()
+    q, k, v, do, _ = _inputs(90, 2, 2, 64)
+    want = _run(q, k, v, do, [90])
+    leaves = [(t.float() if n in wide else t).detach().requires_grad_()
+              for n, t in zip("qkv", (q, k, v))]
+    with torch.autocast("cuda", dtype=dtype):
+        o = FD.packed_causal_attention(
+            *leaves, FD.PackedSequences([90], device="cuda"))
+    assert torch.equal(o.detach(), want["o"])
+    for leaf, grad, name in zip(leaves, torch.autograd.grad(o, leaves, do),
+                                ("dq", "dk", "dv")):
+        assert grad.dtype == leaf.dtype
+        assert torch.equal(grad, want[name].to(grad.dtype))
