@@ -382,7 +382,8 @@ __device__ inline float pa_bias(unsigned entry, int is_bf16) {
 // sum's rounding drops of the score stays in the exponent.  Up to 2^14 that
 // is 2^-11 at most, a tenth of the weights' own step in bf16; beyond 2^30 it
 // could be the score itself, without a maximum taken off.  There each score
-// is rounded with the bias before the maximum is.
+// is rounded with the bias before the maximum is, as in tiles of several
+// biases: one of 4001, 12 heads of 64, forward 54 -> 67 us.
 __device__ inline bool pa_moderate(float x) { return fabsf(x) <= 16384.f; }
 
 __device__ inline const __bf16* pa_at(const PaTensor& t, long row, int head) {

@@ -27,8 +27,8 @@
 // 128 over 8, 1880 us (730 TFLOP/s by the formula's 5 products, 1020 by
 // the 7 performed); seven of 8192 in all, 16 heads over 4, 290 us; eight
 // of 512, 92 us; 20 of 35, 2 heads of 100, 26 us.  With a bias and its
-// gradient: five of 4096 in all, 16 heads of 64, 111 us; one of 4001, 12
-// heads, 173.  Bound by the
+// gradient: five of 4096 in all, 16 heads of 64, 112 us; one of 4001, 12
+// heads, 180; one of 8192, 16 heads of 128 over 2, 1324.  Bound by the
 // matrix units where sequences are long, else by the longest workgroup:
 // the key kernel holds 128 keys for all heads of a group, so it is cut
 // finer than the others.

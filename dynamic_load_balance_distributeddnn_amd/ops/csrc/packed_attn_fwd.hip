@@ -14,8 +14,8 @@
 // 32 rows a wave let one lane's registers hold a row's scores, 64 keys a
 // step are two score tiles to overlap with their exponentials, and two
 // buffers of keys and values of 128 leave room for two workgroups a CU.
-// Measured: one sequence of 8192, 32 heads of 128 over 8, 535 us, 1030
-// TFLOP/s where a plain product of 8192 x 8192 x 8192 reaches 1190; seven
+// Measured: one sequence of 8192, 32 heads of 128 over 8, 498 to 535 us, 1030
+// to 1100 TFLOP/s where a plain product of 8192 x 8192 x 8192 reaches 1190; seven
 // of 8192 in all, 16 heads over 4, 78 us, 780 TFLOP/s; eight of 512, 21 us;
 // 20 of 35, 2 heads of 100, 9 us.  Bound by the matrix units and the
 // exponentials that share the issue with them where sequences are long
@@ -252,8 +252,10 @@ pa_fwd_kernel(const PaFwd p, const BiasArg bias) {
   // to more than 2^16, which fp32 and the bf16 weights (their step is
   // relative) carry without loss.  So no tile looks for its maximum (one of
   // 8192, 32 heads of 128 over 8: 544 -> 532 us).  False, with nothing
-  // done, where they did; the wave then goes on with any_tile, which has as
-  // many barriers.
+  // done, where they did; the wave then takes any_tile, which has as many
+  // barriers, to its end: with keys that grow to six times along the
+  // sequence 521 -> 555 us, and with a bias of -inf from 113 on, where most
+  // rows have no weight in their first tile, 53 -> 73 (4001, 12 heads of 64).
   auto whole_tile = [&](int t) PA_INLINE {
     const int k0 = t * PA_STEP, buf = t & 1;
     const bool more = t + 1 < it.end;

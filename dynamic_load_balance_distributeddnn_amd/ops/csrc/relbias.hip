@@ -9,8 +9,10 @@
 // elements once and are bound by memory, so both move them in vectors of
 // 16 bytes, N elements.  Measured in bf16: 32 heads of 4096 x 4096 166 us
 // forward (6.4 TB/s; a fill writes 6.85), 219 us backward alone (4.9 TB/s;
-// a bare read of as much 6.2); 16 of 2048 x 2048 26 us (5.2 TB/s); the
-// smallest 4 and 6 us, of which a launch is most.
+// a bare read of as much 6.2); 16 of 2048 x 2048 26 us (5.2 TB/s) and 38 us,
+// of 2047 x 2047 forward 46: a row of 257 vectors takes a second strip of
+// workgroups for the last; the smallest 4 and 6 us, of which a launch is
+// most.
 #include <hip/hip_fp16.h>
 
 #include <type_traits>
@@ -360,8 +362,8 @@ static void rb_bwd_shape(const RbArgs& a, int n, int* rows, long* strips,
                          long* blocks) {
   // About 12 waves a CU: 16 run at a time, and a last few alone would cost
   // as much as the first.  32 heads of 4096 x 4096 in bf16: 219 us (4.9
-  // TB/s), with 64 rows a wave 270; 16 of 2047 x 2047: 45, with twice the
-  // waves 55.
+  // TB/s), with 64 rows a wave 270; 16 of 2047 x 2047: 38, with twice the
+  // waves 55 where once took 45.
   const long span = 64 * n;
   const long all = (a.H * rb_div(a.K, span) * a.Q / (12 * 256) + 8) / 8 * 8;
   *rows = (int)(all > 512 ? 512 : all);

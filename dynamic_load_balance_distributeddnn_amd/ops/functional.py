@@ -202,9 +202,10 @@ def relative_position_bias(table, q_len, k_len, max_distance=128,
     """Learned bias by bucketed distance: [nhead, q_len, k_len].
 
     out[h, i, j] = table[bucket(i + k_len - q_len - j), h] with ``table``
-    [num_buckets, nhead] (bf16, fp16 or fp32; the result has its type, the
-    autocast type under autocast).  The queries are the last ``q_len`` of
-    the ``k_len`` positions, so one generated token is ``q_len=1``.
+    [num_buckets, nhead] (bf16, fp16 or fp32; the result has its type, or
+    the autocast type where an fp32 one is read under autocast on the GPU).
+    The queries are the last ``q_len`` of the ``k_len`` positions, so one
+    generated token is ``q_len=1``.
 
     Half of the buckets hold one distance each, the others divide the
     logarithm up to ``max_distance`` evenly, and the last takes all that is
@@ -254,14 +255,20 @@ def packed_causal_attention(q, k, v, packing, scale=None, bias_table=None,
     ``bias_table`` [num_buckets, nhead] adds ``relative_position_bias`` of
     it to the scaled scores without forming the grid; entries of -inf take
     their distances out, and a row left with nothing is zeros (finite ones
-    beyond 1e37 count as 1e37 on the GPU).  ``scale``
-    defaults to d ** -0.5.  What a masked position holds, an infinity or
-    NaN even, does not reach a row that does not see it.
+    beyond 1e37 count as 1e37 on the GPU).  ``scale`` defaults to d ** -0.5.
+
+    What a position ahead of a row or in another sequence holds, an
+    infinity or NaN even, does not reach that row.  Keys and values at
+    distances that the bias takes out have to be numbers: their weight is
+    0, and 0 times an infinity is NaN.
 
     On the GPU: bfloat16 (fp32 is cast to it under autocast, whatever type
-    that names), d <= 128; sums,
-    softmax statistics and the gradients' sums are fp32, and results do
-    not change from run to run.  The table may be fp32 or bfloat16.
+    that names), d <= 128; sums, softmax statistics and the gradients' sums
+    are fp32, and results do not change from run to run.  The table may be
+    fp32 or bfloat16.  Scores are fp32 as well and move a weight by 2**-24
+    of their size: gradients want scaled scores below 1e5, where that
+    reaches bfloat16's own rounding, and from 1e8 on results are no longer
+    sure to be numbers.
     """
     if q.is_cuda and torch.is_autocast_enabled("cuda"):
         q, k, v = (t.to(torch.bfloat16) if t.dtype == torch.float32 else t

@@ -80,8 +80,11 @@ class PackedSequences:
         seq, tile = self._tiles
         steps = -(-np.minimum((tile + 1) * TILE_ROWS, self._n[seq]) // 64)
         total = int(steps.sum()) * heads
-        # 512 workgroups run at a time, so the longest tile is what a launch
-        # takes at least.  Cutting costs a trip of the sums through memory:
+        # The longest tile is what a launch takes at least.  The limits count
+        # on 512 workgroups at a time, which is right for heads of over 64;
+        # of smaller ones 768 to 1024 fit, and places stay empty: one of 4001,
+        # 12 heads of 64 with a bias, is 576 chunks and takes as long as the
+        # longest.  Cutting costs a trip of the sums through memory:
         # one sequence of 4001, 12 heads of 64, forward 73 -> 50 us where
         # the longest is 2.7 times a place's share, but seven packed ones,
         # 16 heads of 128 over 4, 79 -> 85 where it is 1.3 times, and six of
