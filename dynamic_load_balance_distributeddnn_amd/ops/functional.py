@@ -306,8 +306,9 @@ def packed_causal_attention(q, k, v, packing, scale=None, bias_table=None,
         from . import native
         return native.packed_causal_attention(q, k, v, packing, scale,
                                               bias_table, starts)
-    return _packed_attention_plain(q, k, v, packing, scale, bias_table,
-                                   max_distance)
+    with torch.autocast(device.type, enabled=False):  # its sums are fp32
+        return _packed_attention_plain(q, k, v, packing, scale, bias_table,
+                                       max_distance)
 
 
 def _refuse_packed_attention(q, k, v, packing):

@@ -31,8 +31,8 @@ class PackedSequences:
 
     For each head layout it is used with it keeps work lists on the device,
     of the query tiles and, for gradients, of the key tiles.  A list's tiles
-    times the heads have to be below 2**24 (a million sequences of one row
-    with 16 heads are too many).
+    times the heads have to be below 2**24 (2**20 sequences of one row with
+    16 heads are too many).
     """
 
     def __init__(self, lengths, device=None):

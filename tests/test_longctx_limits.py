@@ -31,3 +31,20 @@ def test_more_tiles_than_a_launch_takes():
     for rows, chunks, slots in pack.host_work(15, 15):
         assert rows.shape == (2 ** 20, 8)
         assert (chunks, slots) == (2 ** 20, 0)
+
+
+@pytest.mark.parametrize("buckets", [0, 8])
+def test_autocast_leaves_the_statistics_in_32_bits(buckets):
+    """The composition's own products are not cast on the CPU."""
+    gen = torch.Generator().manual_seed(0)
+    q, k, v = (torch.randn(70, 2, 16, generator=gen) for _ in range(3))
+    table = torch.randn(buckets, 2, generator=gen) if buckets else None
+    pack = FD.PackedSequences([60, 10])
+    for dtype in (torch.float32, torch.bfloat16):
+        given = [t.to(dtype) for t in (q, k, v)]
+        want = FD.packed_causal_attention(*given, pack, bias_table=table,
+                                          max_distance=20)
+        with torch.autocast("cpu", dtype=torch.bfloat16):
+            got = FD.packed_causal_attention(*given, pack, bias_table=table,
+                                             max_distance=20)
+        assert got.dtype == dtype and torch.equal(got, want)
